@@ -38,6 +38,7 @@ class DeviceInfo(ctypes.Structure):
     ]
 
 
+_I64P = ctypes.POINTER(c_int64)
 _A16_ARGS = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
              c_int, c_int, c_void_p, c_size_t, c_void_p]
 
@@ -81,6 +82,11 @@ SIGNATURES = {
                                             c_int, c_int, c_void_p]),
     "asrq_decode_grouped_attention": (c_int, [c_void_p] * 9 + [c_int64, c_int, c_int, c_int, c_int64, ctypes.c_float, ctypes.c_float, c_int,
                                               c_void_p]),
+    "asrq_beam_select": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int64] * 4 + [c_int, c_void_p]),
+    "asrq_beam_reorder": (c_int, [c_void_p] * 3 + [c_int64] * 7 + [c_void_p]),
+    "asrq_cross_attention": (c_int, [c_void_p, _I64P] * 3 + [c_void_p] * 2 + [c_int64] * 2 + [c_int] * 3 + [c_int64, ctypes.c_float, c_int, c_void_p]),
+    "asrq_prefix_attention": (c_int, [c_void_p, _I64P] * 3 + [c_void_p] + [c_void_p, _I64P] * 2 + [c_void_p, c_int64, c_void_p] + [c_int64] * 2 + [c_int] * 3 +
+                              [c_int64] * 2 + [ctypes.c_float, c_int, c_void_p]),
     "asrq_dense_head": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
     "asrq_rtn_pack": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                               c_void_p]),

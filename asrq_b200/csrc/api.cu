@@ -57,6 +57,16 @@ int bias_add_transposed(const void* x, const void* conv, const void* bias, void*
 int half_step(const void* x, const void* y, void* out, int64_t n, int dtype, cudaStream_t stream);
 int dense_head(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int dtype, int sm_count, cudaStream_t stream);
 int argmax_rows(const void* y, long long* tok, long long* ids, const long long* pos, void* scratch, int64_t B, int64_t N, int dtype, cudaStream_t stream);
+bool beam_select_fits(int64_t K, int64_t V);
+int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores, const uint8_t* finished, int64_t eos, float* out_scores,
+                long long* parents, long long* tokens, uint8_t* out_finished, int64_t B, int64_t K, int64_t V, int64_t n, int dtype, int sm_count,
+                cudaStream_t stream);
+int beam_reorder(void* cache, const long long* parents, const long long* length_dev, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
+                 int64_t max_len, int64_t pos_bytes, cudaStream_t stream);
+int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
+                   const void* k2, const int64_t* k2s, const void* v2, const int64_t* v2s, const long long* lengths2, bool lengths2_many, void* out,
+                   int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, float scale, int dtype, int sm_count,
+                   cudaStream_t stream);
 int hadamard_quant_int4(const void* x, uint8_t* qa, float* sa, int64_t M, int64_t K, int hadamard, int dtype,
                         int out_int8, cudaStream_t stream);
 int w4a4_linear_tc(const void* x, const uint8_t* qw, const void* sw, const void* bias, void* y, int64_t M, int64_t N,
@@ -709,6 +719,102 @@ int asrq_decode_grouped_attention(const void* qkv, const void* q_weight, const v
   if (B == 0) return ASRQ_OK;
   return decode_grouped_attention(qkv, q_weight, k_weight, cos_table, sin_table, reinterpret_cast<const long long*>(pos_device), k_cache, v_cache, out, B,
                                   n_kv_heads, max_len, eps, scale, dtype, f->sm_count, static_cast<cudaStream_t>(stream));
+}
+
+int asrq_beam_select(const void* logits, int64_t utterance_stride, int64_t beam_stride, const float* scores, const uint8_t* finished, int64_t eos,
+                     float* out_scores, int64_t* parents, int64_t* tokens, uint8_t* out_finished, int64_t B, int64_t K, int64_t V, int64_t n,
+                     int dtype, void* stream) {
+  last_error().clear();
+  if (!logits || !scores || !out_scores || !parents || !tokens || (finished && !out_finished))
+    return fail(ASRQ_ERR_NULL, "asrq_beam_select: logits, scores and the outputs must not be NULL; finished needs out_finished");
+  if (dtype != ASRQ_F16 && dtype != ASRQ_BF16) return fail(ASRQ_ERR_DTYPE, "asrq_beam_select: dtype %d", dtype);
+  if (B < 0 || B > (1 << 24) || K <= 0 || V <= 0 || n <= 0 || n > K * V || beam_stride < 0 || utterance_stride < 0)
+    return fail(ASRQ_ERR_SHAPE, "asrq_beam_select: B=%lld K=%lld V=%lld n=%lld (at most K * V) strides %lld, %lld", (long long)B, (long long)K, (long long)V,
+                (long long)n, (long long)utterance_stride, (long long)beam_stride);
+  if (finished && (eos < 0 || eos >= V)) return fail(ASRQ_ERR_SHAPE, "asrq_beam_select: eos=%lld of %lld tokens", (long long)eos, (long long)V);
+  if (K > 32 || n > 32 || !beam_select_fits(K, V))
+    return fail(ASRQ_ERR_LIMIT, "asrq_beam_select: K=%lld n=%lld (at most 32) V=%lld (at most 65536 values for each of the 128 / K segments of a row)", (long long)K,
+                (long long)n, (long long)V);
+  if (reinterpret_cast<uintptr_t>(logits) % 2) return fail(ASRQ_ERR_ALIGN, "asrq_beam_select: logits must be 2-byte aligned");
+  const DeviceFacts* f;
+  int rc;
+  if ((rc = device_facts(&f))) return rc;
+  if (B == 0) return ASRQ_OK;
+  return beam_select(logits, utterance_stride, beam_stride, scores, finished, eos, out_scores, reinterpret_cast<long long*>(parents),
+                     reinterpret_cast<long long*>(tokens), out_finished, B, K, V, n, dtype, f->sm_count, static_cast<cudaStream_t>(stream));
+}
+
+int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length_device, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
+                      int64_t max_len, int64_t position_bytes, void* stream) {
+  last_error().clear();
+  if (!cache || !parents) return fail(ASRQ_ERR_NULL, "asrq_beam_reorder: cache and parents must not be NULL");
+  if (L < 0 || B < 0 || K <= 0 || heads <= 0 || max_len <= 0 || position_bytes <= 0 || position_bytes % 16 || position_bytes > (1 << 20) ||
+      max_len > (int64_t(1) << 31) || L > (1 << 24) || B > (1 << 24) || heads > (1 << 16) || L * B > (1 << 30) || L * B * heads > 0x7fffffff)
+    return fail(ASRQ_ERR_SHAPE, "asrq_beam_reorder: L=%lld B=%lld K=%lld heads=%lld max_len=%lld position_bytes=%lld (a multiple of 16)", (long long)L,
+                (long long)B, (long long)K, (long long)heads, (long long)max_len, (long long)position_bytes);
+  if (K > 32) return fail(ASRQ_ERR_LIMIT, "asrq_beam_reorder: K=%lld (at most 32)", (long long)K);
+  if (!aligned16(cache)) return fail(ASRQ_ERR_ALIGN, "asrq_beam_reorder: cache must be 16-byte aligned");
+  const DeviceFacts* f;
+  int rc;
+  if ((rc = device_facts(&f))) return rc;
+  if (L == 0 || B == 0 || K == 1) return ASRQ_OK;
+  return beam_reorder(cache, reinterpret_cast<const long long*>(parents), reinterpret_cast<const long long*>(length_device), length, L, B, K, heads, max_len,
+                      position_bytes, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+// What the two attentions of shared keys have in common
+int check_rows(const char* who, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* out, int64_t B,
+               int64_t R, int nq, int nkv, int hd, int64_t keys, int dtype) {
+  if (!q || !out || !qs || !ks || !vs || (keys > 0 && (!k || !v))) return fail(ASRQ_ERR_NULL, "%s: q, k, v, out and the strides must not be NULL", who);
+  if (dtype != ASRQ_F16 && dtype != ASRQ_BF16) return fail(ASRQ_ERR_DTYPE, "%s: dtype %d", who, dtype);
+  if (B < 0 || R < 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq > (1 << 16) || (hd != 64 && hd != 128) || keys < 0 || keys > 0x7fffffff || R > (1 << 24) ||
+      B > (1 << 24) || R * (nq / nkv) > (1 << 24) || B * nkv * ((R * (nq / nkv) + 15) / 16) > (1 << 27))
+    return fail(ASRQ_ERR_SHAPE, "%s: B=%lld rows=%lld heads=%d/%d head_dim=%d (64 or 128) keys=%lld", who, (long long)B, (long long)R, nq, nkv, hd, (long long)keys);
+  for (const int64_t* s : {qs, ks, vs})
+    if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[0] % 8 || s[1] % 8 || s[2] % 8)
+      return fail(ASRQ_ERR_ALIGN, "%s: strides %lld, %lld, %lld (multiples of 8)", who, (long long)s[0], (long long)s[1], (long long)s[2]);
+  for (const void* x : {q, keys > 0 ? k : q, keys > 0 ? v : q})
+    if (!aligned16(x)) return fail(ASRQ_ERR_ALIGN, "%s: q, k and v must be 16-byte aligned", who);
+  return ASRQ_OK;
+}
+}  // namespace
+
+int asrq_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         const int64_t* lengths, void* out, int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t keys, float scale,
+                         int dtype, void* stream) {
+  last_error().clear();
+  int rc = check_rows("asrq_cross_attention", q, q_strides, k, k_strides, v, v_strides, out, B, R, n_q_heads, n_kv_heads, head_dim, keys, dtype);
+  if (rc) return rc;
+  const DeviceFacts* f;
+  if ((rc = device_facts(&f))) return rc;
+  if (B == 0 || R == 0) return ASRQ_OK;
+  return rows_attention(q, q_strides, k, k_strides, v, v_strides, reinterpret_cast<const long long*>(lengths), nullptr, nullptr, nullptr, nullptr, nullptr, false, out,
+                        B, R, n_q_heads, n_kv_heads, head_dim, keys, 0, scale, dtype, f->sm_count, static_cast<cudaStream_t>(stream));
+}
+
+int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k_prefix, const int64_t* k_prefix_strides, const void* v_prefix,
+                          const int64_t* v_prefix_strides, const int64_t* prefix_lengths, const void* k_suffix, const int64_t* k_suffix_strides,
+                          const void* v_suffix, const int64_t* v_suffix_strides, const int64_t* suffix_lengths, int64_t n_suffix_lengths, void* out, int64_t B,
+                          int64_t K, int n_q_heads, int n_kv_heads, int head_dim, int64_t prefix_keys, int64_t suffix_keys, float scale, int dtype,
+                          void* stream) {
+  last_error().clear();
+  int rc = check_rows("asrq_prefix_attention", q, q_strides, k_prefix, k_prefix_strides, v_prefix, v_prefix_strides, out, B, K, n_q_heads, n_kv_heads, head_dim,
+                      prefix_keys, dtype);
+  if (!rc)
+    rc = check_rows("asrq_prefix_attention", q, q_strides, k_suffix, k_suffix_strides, v_suffix, v_suffix_strides, out, B, K, n_q_heads, n_kv_heads, head_dim,
+                    suffix_keys, dtype);
+  if (rc) return rc;
+  if (!suffix_lengths) return fail(ASRQ_ERR_NULL, "asrq_prefix_attention: suffix_lengths must not be NULL");
+  if (n_suffix_lengths != 1 && n_suffix_lengths != B * K)
+    return fail(ASRQ_ERR_SHAPE, "asrq_prefix_attention: %lld suffix lengths (1 or B * K = %lld)", (long long)n_suffix_lengths, (long long)(B * K));
+  const DeviceFacts* f;
+  if ((rc = device_facts(&f))) return rc;
+  if (B == 0 || K == 0) return ASRQ_OK;
+  return rows_attention(q, q_strides, k_prefix, k_prefix_strides, v_prefix, v_prefix_strides, reinterpret_cast<const long long*>(prefix_lengths),
+                        suffix_keys > 0 ? k_suffix : nullptr, k_suffix_strides, v_suffix, v_suffix_strides, reinterpret_cast<const long long*>(suffix_lengths),
+                        n_suffix_lengths != 1, out, B, K, n_q_heads, n_kv_heads, head_dim, prefix_keys, suffix_keys, scale, dtype, f->sm_count,
+                        static_cast<cudaStream_t>(stream));
 }
 
 int asrq_dense_head(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {

@@ -305,6 +305,58 @@ int asrq_decode_grouped_attention(const void* qkv, const void* q_weight, const v
                                   int head_dim, int64_t max_len, float eps, float scale, int dtype, void* stream);
 
 /*
+ * Decoding with several hypotheses (beams) per utterance: the selection of a step.  Over the K beams and V tokens of an utterance
+ *   s[k, v] = scores[k] + logits[k, v] - log sum_v' exp logits[k, v'],
+ * and the n largest with their beam (parents) and token, descending, of equal ones the lowest k * V + v first (the logits of a beam decide
+ * before s is rounded).  s is computed in 64 bits and returned in 32.
+ *   logits      beam k of utterance b at logits + b * utterance_stride + k * beam_stride, V contiguous values of `dtype`, at any value's address;
+ *   scores      B x K; a beam whose score is not finite is no hypothesis: its continuations have -inf (at the first step all but one beam);
+ *               so has one whose logits hold a NaN, a +inf or nothing above -inf;
+ *   finished    B x K bytes, or NULL: a beam that has ended goes on with the token eos at its own score and with nothing else (-inf); its logits are not
+ *               read.  out_finished (B x n): 1 where the parent had ended or the token is eos;
+ *   out_scores, parents, tokens   B x n.
+ * K and n at most 32, V at most 65536 * floor(128 / K).  No scratch, no state between calls.
+ */
+int asrq_beam_select(const void* logits, int64_t utterance_stride, int64_t beam_stride, const float* scores, const uint8_t* finished, int64_t eos,
+                     float* out_scores, int64_t* parents, int64_t* tokens, uint8_t* out_finished, int64_t B, int64_t K, int64_t V, int64_t n,
+                     int dtype, void* stream);
+
+/*
+ * The caches of the beams follow the hypotheses that were kept: cache[l, b * K + k, h, t] = cache[l, b * K + parents[b, k], h, t] for every l < L and
+ * h < heads and the positions t < length, in place; positions from `length` on stay as they are.  cache: L x (B * K) x heads x max_len
+ * positions of position_bytes (a multiple of 16), any type, 16-byte aligned.  parents: B x K; a parent outside 0..K-1 leaves its beam as it is.
+ * The length is read from length_device when that is not NULL and is the argument otherwise, and is cut to 0..max_len.  K at most 32.
+ * A kernel that reads the cache ahead of the stream dependency (asrq_decode_self_attention_settled,
+ * asrq_decode_grouped_attention) needs an ordinary kernel or copy between this call and its own.
+ */
+int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length_device, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
+                      int64_t max_len, int64_t position_bytes, void* stream);
+
+/*
+ * Attention of R query rows of every utterance (the beams of a step, the tokens of a prompt) over its encoder states:
+ * out[b, r, h] = softmax(scale * q[b, r, h] . k[b, t, h'])_t . v[b, t, h'], t < lengths[b], h' = h / (n_q_heads / n_kv_heads).
+ *   q, q_strides   values between utterances, rows and heads;  k, v and theirs: between utterances, heads and positions; multiples of 8;
+ *   lengths        B, cut to 0..keys, or NULL for `keys` everywhere; nothing past an utterance's length is read; a row without keys is zero;
+ *   out            B x R x n_q_heads x head_dim, contiguous.
+ * head_dim 64 or 128; q, k and v 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation.
+ */
+int asrq_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         const int64_t* lengths, void* out, int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t keys, float scale,
+                         int dtype, void* stream);
+
+/*
+ * Attention of one decoding step of K beams (or samples) of every utterance that share a prompt: over the prompt's keys, held once
+ * for the utterance, and the beam's own behind them.  q[b, k]: K rows; prefix keys and values at strides between utterances, heads and positions,
+ * prefix_lengths (B, or NULL for prefix_keys everywhere) of them; suffix keys and values of B * K sequences at strides between sequences, heads and
+ * positions, suffix_lengths of them: one for all or B * K, device memory.  Otherwise as asrq_cross_attention; either part may be empty.
+ */
+int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k_prefix, const int64_t* k_prefix_strides, const void* v_prefix,
+                          const int64_t* v_prefix_strides, const int64_t* prefix_lengths, const void* k_suffix, const int64_t* k_suffix_strides,
+                          const void* v_suffix, const int64_t* v_suffix_strides, const int64_t* suffix_lengths, int64_t n_suffix_lengths, void* out, int64_t B,
+                          int64_t K, int n_q_heads, int n_kv_heads, int head_dim, int64_t prefix_keys, int64_t suffix_keys, float scale, int dtype,
+                          void* stream);
+
+/*
  * The floating-point output head of a decoding step: y[M, N] = x[M, K] . w[N, K]^T, all of the 16-bit type `dtype`,
  * fp32 accumulation, for M <= 32 tokens and a vocabulary-sized N (any N >= 1).  The reference keeps these layers as
  * nn.Linear (proj_out, asrq/models/transformers/whisper.py:268; lm_head, asrq/models/nemo/canary_qwen.py:179); after
