@@ -138,3 +138,64 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
                       v_suffix.data_ptr(), _strides(v_suffix, 0, 1, 2), suffix_lengths.data_ptr(), suffix_lengths.numel(), out.data_ptr(), B, K, Hq, Hkv, hd, P, M,
                       hd ** -0.5 if scale is None else float(scale), dt, torch.cuda.current_stream(q.device).cuda_stream)
     return out
+
+
+def end_token(config, eos=None):
+    """The token that ends a hypothesis: the one given, else the configuration's (the first of several), None where it has none."""
+    eos = getattr(config, "eos_token_id", None) if eos is None else eos
+    eos = next(iter(eos), None) if isinstance(eos, (list, tuple)) else eos
+    return None if eos is None else int(eos)
+
+
+class BeamState:
+    """The hypotheses of a batch while they grow: B utterances, K beams each, ``steps`` tokens.  :meth:`start` takes the logits of the prompt's last position
+    (one hypothesis per utterance), :meth:`advance` those of a step; both leave the next tokens in ``tok`` (B * K,).  Everything lives in static
+    buffers and every index on the device, so :meth:`advance` may be captured.  An ended hypothesis is carried along with the end token
+    (``eos``; None: nothing ends) at its score; what is kept of a step are tokens and parents, from which :meth:`hypotheses` reads the sequences
+    back."""
+
+    def __init__(self, batch: int, beams: int, steps: int, eos, device):
+        self.B, self.K, self.steps, self.eos = batch, beams, steps, eos
+        self.tok = torch.zeros(batch * beams, dtype=torch.long, device=device)
+        self.at = torch.zeros(1, dtype=torch.long, device=device)  # tokens so far
+        self.scores = torch.zeros(batch, beams, dtype=torch.float32, device=device)
+        self.finished = torch.zeros(batch, beams, dtype=torch.bool, device=device)
+        self.tokens = torch.zeros(steps, batch, beams, dtype=torch.long, device=device)
+        self.parents = torch.zeros(steps, batch, beams, dtype=torch.long, device=device)
+
+    def start(self, logits: torch.Tensor) -> None:
+        """``logits`` (B, V): the K best tokens of every utterance open its beams (the vocabulary has as many)."""
+        scores, parents, tokens = beam_select(logits.view(self.B, 1, -1), torch.zeros(self.B, 1, device=logits.device), self.K)
+        self.tokens[0], self.parents[0] = tokens, parents
+        self.scores.copy_(scores)
+        if self.eos is not None:
+            self.finished.copy_(tokens == self.eos)
+        self.tok.copy_(tokens.view(-1))
+        self.at.fill_(1)
+
+    def advance(self, logits: torch.Tensor, caches, length: torch.Tensor) -> None:
+        """``logits`` (B * K, V): selects, and lets the ``caches`` (each as :func:`beam_reorder` takes it) follow up to ``length`` positions."""
+        picked = beam_select(logits.view(self.B, self.K, -1), self.scores, finished=None if self.eos is None else self.finished, eos=self.eos)
+        scores, parents, tokens = picked[:3]
+        for cache in caches:
+            beam_reorder(cache, parents, length)
+        self.scores.copy_(scores)
+        if self.eos is not None:
+            self.finished.copy_(picked[3])
+        self.tok.copy_(tokens.view(-1))
+        self.tokens.index_copy_(0, self.at, tokens.unsqueeze(0))
+        self.parents.index_copy_(0, self.at, parents.unsqueeze(0))
+        self.at.add_(1)
+
+    def hypotheses(self, length_penalty: float = 1.0):
+        """``(ids, scores)``: ids (B, K, steps), the end token behind the end; scores (B, K): the sum of the log probabilities over the number of
+        tokens, the end token among them, to the power of ``length_penalty``.  Best first."""
+        ids = torch.empty(self.B, self.K, self.steps, dtype=torch.long, device=self.tok.device)
+        beam = torch.arange(self.K, device=self.tok.device).expand(self.B, self.K)
+        for s in range(self.steps - 1, -1, -1):
+            ids[:, :, s] = self.tokens[s].gather(1, beam)
+            beam = self.parents[s].gather(1, beam)
+        length = ids.new_full((self.B, self.K), self.steps) if self.eos is None else ((ids == self.eos).cumsum(-1) <= (ids == self.eos)).sum(-1)  # up to the first end token
+        scores = self.scores / length.to(torch.float32) ** length_penalty
+        order = torch.sort(scores, dim=1, descending=True, stable=True)
+        return ids.gather(1, order.indices.unsqueeze(-1).expand_as(ids)), order.values

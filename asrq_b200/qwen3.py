@@ -22,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import packing
+from .beam import BeamState, end_token, prefix_attention
 from .convert import linearq_from_linear
 from .linear import (PRE_RMSNORM, PRE_SILU_MUL, LinearQ, add_rmsnorm, argmax_rows, calls_only_linearq, decode_grouped_attention, dense_head,
                      linear_after, qk_norm_rope, silu_mul)
@@ -350,3 +351,76 @@ class Qwen3Engine:
             return first.view(-1, 1)
         rest = self.decode(steps - 1, use_graph=use_graph)
         return torch.cat([first.view(-1, 1), rest], dim=1)
+
+    # ---- beam search --------------------------------------------------------------------------
+    def _beam_step(self, st: dict) -> None:
+        """One token for every beam: a row of the batch is a beam.  The prompt's keys stay where :meth:`prefill` wrote them, once per sequence; a beam's
+        own positions have caches of their own, which follow the selection."""
+        beams, pos, T = st["beams"], st["pos"], st["T"]
+        rows = beams.B * beams.K
+        x, delta = self.embed[beams.tok], None
+        st["len"].copy_(pos + 1)
+        cos, sin = self.cos[T:], self.sin[T:]
+        for i, L in enumerate(self.layers):
+            ks, vs = st["kv"][i]
+            x, h = add_rmsnorm(x, delta, L["ln1"], self.eps)
+            q = qk_norm_rope(L["qkv"](h), L["qn"], L["kn"], cos, sin, ks, vs, pos, rows, 1, self.nq, self.nkv, self.eps)
+            a = prefix_attention(q.view(beams.B, beams.K, self.nq, self.hd), self.kc[i][:, :, :T], self.vc[i][:, :, :T], ks, vs, st["len"])
+            x, h = add_rmsnorm(x, L["o"](a.view(rows, -1)), L["ln2"], self.eps)
+            delta = L["down"](silu_mul(L["gu"](h)))
+        dense_head(self._final(x, delta), self.head, out=st["logits"])
+        pos.add_(1)
+        kv = st["kv"]
+        beams.advance(st["logits"], [kv.view(-1, rows, *kv.shape[3:])], pos)
+
+    @torch.no_grad()
+    def beam_search(self, inputs_embeds: torch.Tensor, steps: int, beams: int = 5, eos: Optional[int] = None, length_penalty: float = 1.0, use_graph: bool = True):
+        """Beam search over ``steps`` tokens behind the prompt (B, T, H).  Returns ``(ids, scores)``: ids (B, beams, steps), best first, the end token
+        (``eos``, the configuration's where None) behind the end; scores (B, beams), the log probability over length ** ``length_penalty``.
+        All ``steps`` run."""
+        B, T, _ = inputs_embeds.shape
+        if steps < 1 or not 1 <= beams <= 32:
+            raise ValueError(f"{steps} steps, {beams} beams (1 to 32)")
+        eos = end_token(self.cfg, eos)
+        with torch.cuda.device(self.device):
+            self.prefill(inputs_embeds, steps)
+            key = (B, T, steps, beams, eos, self.kc[0].data_ptr())
+            st = getattr(self, "_beam", None)
+            if st is None or st["key"] != key:
+                st = dict(key=key, T=T, beams=BeamState(B, beams, steps, eos, self.device), graph=None, caches=(self.kc, self.vc),
+                          kv=torch.zeros(len(self.layers), 2, B * beams, self.nkv, steps, self.hd, device=self.device, dtype=self.dtype),
+                          pos=torch.zeros(1, dtype=torch.long, device=self.device), len=torch.zeros(1, dtype=torch.long, device=self.device),
+                          logits=torch.empty(B * beams, self.head.shape[0], device=self.device, dtype=self.dtype))
+                self._beam = st
+            st["beams"].start(self.last_logits)
+            st["pos"].zero_()
+            if use_graph and steps > 1:
+                self._beam_graph(st)
+            for _ in range(steps - 1):
+                if use_graph:
+                    st["graph"].replay()
+                else:
+                    self._beam_step(st)
+            return st["beams"].hypotheses(length_penalty)
+
+    def _beam_graph(self, st: dict) -> None:
+        ops = _baked_in(self.layers + [self.norm, self.embed, self.head, self.eps, self.cos, self.sin])
+        if st["graph"] is not None and _same(ops, st["ops"]):
+            return
+        beams = st["beams"]
+        state = (beams.tok, beams.scores, beams.finished, beams.tokens, beams.parents)
+        kept = [x.clone() for x in state]
+        side = torch.cuda.Stream(self.device)
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(side):
+            self._beam_step(st)  # warm-up outside the capture
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                self._beam_step(st)
+        torch.cuda.current_stream(self.device).wait_stream(side)
+        for x, old in zip(state, kept):
+            x.copy_(old)
+        beams.at.fill_(1)
+        st["pos"].zero_()
+        st["graph"], st["ops"] = g, ops

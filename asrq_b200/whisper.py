@@ -30,6 +30,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import packing
+from .beam import BeamState, cross_attention, end_token
 from .convert import linearq_from_linear
 from .linear import PRE_LAYERNORM, LinearQ, add_layernorm, argmax_rows, decode_cross_attention, decode_self_attention, dense_head, linear_after
 
@@ -544,6 +545,111 @@ class WhisperEngine:
         with torch.cuda.device(self.device):
             enc = self.encode(input_features)
             return self.decode(enc, steps, use_graph=use_graph)
+
+    # ---- beam search --------------------------------------------------------------------------
+    def _heads(self, x, heads):
+        return x.view(*x.shape[:-1], heads, -1)
+
+    def _beam_prompt(self, st: dict, prompt: torch.Tensor, lengths) -> torch.Tensor:
+        """The prompt (B, T) of every utterance at once: its keys and values into the caches of all of its beams; the last position's logits (B, V)."""
+        b, t = prompt.shape
+        k_beams, hd, heads = st["beams"].K, self.d // self.heads_d, self.heads_d
+        scaling = hd ** -0.5
+        x = self.embed[prompt] + self.dec_pos[:t]
+        for i, L in enumerate(self.dec_layers):
+            q, k, v = (self._split_heads(y, heads) for y in L["qkv"](L["ln1"](x)).split(self.d, dim=-1))
+            kv = st["kv"][i].view(2, b, k_beams, heads, -1, hd)
+            kv[0, :, :, :, :t], kv[1, :, :, :, :t] = k.unsqueeze(1), v.unsqueeze(1)
+            a = F.scaled_dot_product_attention(q, k, v, is_causal=t > 1, scale=1.0 if L["q_folded"] else scaling)
+            x = L["out"].forward_fused(a.transpose(1, 2).reshape(b, t, -1), residual=x)
+            a = cross_attention(self._heads(L["xq"](L["lnx"](x)), heads), *st["cross"][i], lengths=lengths, scale=1.0 if L["xq_folded"] else scaling)
+            x = L["xout"].forward_fused(a.view(b, t, -1), residual=x)
+            x = L["fc2"].forward_fused(L["fc1"].forward_fused(L["ln2"](x), gelu=True), residual=x)
+        return dense_head(self.dec_ln(x[:, -1].contiguous()), self.head)
+
+    def _beam_step(self, st: dict, lengths) -> None:
+        """One token for every beam, on static buffers like :meth:`_step`.  A row of the batch is a beam; the encoder's keys are read once for all
+        beams of an utterance, and the self-attention caches follow the selection."""
+        beams, pos, heads = st["beams"], st["pos"], self.heads_d
+        rows, b = beams.B * beams.K, beams.B
+        scaling = (self.d // heads) ** -0.5
+        x = (self.embed[beams.tok] + self.dec_pos[pos]).unsqueeze(1)
+        for i, L in enumerate(self.dec_layers):
+            a = decode_self_attention(_norm_then(L["ln1"], L["qkv"], x), st["kv"][i], pos, 1.0 if L["q_folded"] else scaling, settled=True).unsqueeze(1)
+            x = L["out"].forward_fused(a, residual=x)
+            q = _norm_then(L["lnx"], L["xq"], x)
+            a = cross_attention(q.view(b, beams.K, heads, -1), *st["cross"][i], lengths=lengths, scale=1.0 if L["xq_folded"] else scaling)
+            x = L["xout"].forward_fused(a.view(rows, 1, -1), residual=x)
+            x = L["fc2"].forward_fused(_norm_then(L["ln2"], L["fc1"], x, gelu=True), residual=x)
+        dense_head(self.dec_ln(x).squeeze(1), self.head, out=st["logits"])
+        pos.add_(1)
+        kv = st["kv"]
+        beams.advance(st["logits"], [kv.view(-1, rows, heads, *kv.shape[4:])], pos)
+
+    @torch.no_grad()
+    def beam_search(self, enc: torch.Tensor, steps: int, beams: int = 5, prompt: Optional[torch.Tensor] = None, enc_lengths: Optional[torch.Tensor] = None,
+                    eos: Optional[int] = None, length_penalty: float = 1.0, use_graph: bool = True):
+        """Beam search over ``steps`` tokens behind ``prompt`` (B, T) (the start token where None), on encoder states (B, S, d) of which the first
+        ``enc_lengths`` (B,) int64 count (all where None).  Returns ``(ids, scores)``: ids (B, beams, steps), best first, the end token (``eos``, the
+        configuration's where None) behind the end; scores (B, beams), the log probability over length ** ``length_penalty``.  All ``steps`` run."""
+        b, src, _ = enc.shape
+        start = self.cfg.decoder_start_token_id
+        eos = end_token(self.cfg, eos)
+        with torch.cuda.device(self.device):
+            prompt = torch.full((b, 1), start, dtype=torch.long, device=self.device) if prompt is None else prompt.to(device=self.device, dtype=torch.long)
+            t = prompt.shape[1]
+            if steps < 1 or t < 1 or prompt.shape[0] != b or t + steps - 1 > self.dec_pos.shape[0]:
+                raise ValueError(f"a prompt {tuple(prompt.shape)} for {b} utterances and {steps} steps in the model's {self.dec_pos.shape[0]} target positions")
+            if not 1 <= beams <= 32:
+                raise ValueError(f"{beams} beams (1 to 32)")
+            key = (b, src, beams, t + steps, steps, eos, enc_lengths is not None)
+            st = getattr(self, "_beam", None)
+            if st is None or st["key"] != key:
+                hd, nl = self.d // self.heads_d, len(self.dec_layers)
+                xkv = torch.empty(nl, b, src, 2 * self.d, device=self.device, dtype=self.dtype)
+                kv = xkv.view(nl, b, src, 2, self.heads_d, hd)
+                st = dict(key=key, beams=BeamState(b, beams, steps, eos, self.device), graph=None, xkv=xkv, cross=[(kv[i, :, :, 0], kv[i, :, :, 1]) for i in range(nl)],
+                          kv=torch.zeros(nl, 2, b * beams, self.heads_d, t + steps, hd, device=self.device, dtype=self.dtype),
+                          pos=torch.zeros(1, dtype=torch.long, device=self.device), lengths=torch.zeros(b, dtype=torch.long, device=self.device),
+                          logits=torch.empty(b * beams, self.head.shape[0], device=self.device, dtype=self.dtype))
+                self._beam = st
+            lengths = None
+            if enc_lengths is not None:
+                lengths = st["lengths"].copy_(enc_lengths)
+            for i, L in enumerate(self.dec_layers):
+                st["xkv"][i].copy_(L["xkv"](enc))
+            st["beams"].start(self._beam_prompt(st, prompt, lengths))
+            st["pos"].fill_(t)
+            if use_graph and steps > 1:
+                self._beam_graph(st, lengths, t)
+            for _ in range(steps - 1):
+                if use_graph:
+                    st["graph"].replay()
+                else:
+                    self._beam_step(st, lengths)
+            return st["beams"].hypotheses(length_penalty)
+
+    def _beam_graph(self, st: dict, lengths, t: int) -> None:
+        ops = _baked_in(self.dec_layers + [self.embed, self.dec_pos, self.dec_ln, self.head])
+        if st["graph"] is not None and _same(ops, st["ops"]):
+            return
+        beams = st["beams"]
+        state = (beams.tok, beams.scores, beams.finished, beams.tokens, beams.parents)
+        kept = [x.clone() for x in state]  # (the prompt's keys are the same in all beams of an utterance, and later ones are written anew)
+        side = torch.cuda.Stream(self.device)
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(side):
+            self._beam_step(st, lengths)  # warm-up outside the capture
+            side.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                self._beam_step(st, lengths)
+        torch.cuda.current_stream(self.device).wait_stream(side)
+        for x, old in zip(state, kept):
+            x.copy_(old)
+        beams.at.fill_(1)
+        st["pos"].fill_(t)
+        st["graph"], st["ops"] = g, ops
 
 
 def audio_seconds(config, batch: int) -> float:

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import asrq_b200
-from beam_util import check_select
+from tests.beam_util import check_select
 
 DEV = "cuda"
 pytestmark = pytest.mark.gpu

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import asrq_b200
-from beam_util import check_rows
+from tests.beam_util import check_rows
 
 DEV = "cuda"
 pytestmark = pytest.mark.gpu
