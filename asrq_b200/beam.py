@@ -16,6 +16,7 @@ import ctypes
 import torch
 
 from . import _lib
+from . import linear as _linear
 from .linear import _expect, _on_device, _require_cuda_16bit
 
 
@@ -31,6 +32,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int = None, finis
     int64, ``parents`` the beam that goes on.  With ``finished`` (B, K) bool and ``eos``: a finished beam goes on with ``eos`` at its own score
     and nothing else, and the fourth result says which of the new hypotheses have ended.  A beam whose score is not finite (at the first
     step all but one) or whose logits are no distribution (a NaN, a +inf, nothing above -inf) offers its tokens at -inf."""
+    if _linear._native is not None:  # the ordinary case in native code; None where it is not one
+        out = _linear._native.beam_select(logits, scores, scores.shape[-1] if n is None else n, finished, eos)
+        if out is not None:
+            return out
     dt = _require_cuda_16bit(logits, "beam_select")
     _expect(logits.dim() == 3, f"beam_select: logits (B, K, V), got {tuple(logits.shape)}")
     B, K, V = logits.shape
@@ -58,6 +63,8 @@ def beam_reorder(cache: torch.Tensor, parents: torch.Tensor, length) -> torch.Te
     """The beams' caches follow the hypotheses that were kept, in place: ``cache`` (L, B * K, heads, max_len, head_dim), contiguous, of any type with
     16-byte positions; for every utterance b and beam k the positions below ``length`` (an int, or a one-element int64 CUDA tensor)
     become those of beam ``parents[b, k]`` (``parents`` (B, K) int64); a parent that is no beam leaves the row as it is.  Returns ``cache``."""
+    if _linear._native is not None and _linear._native.beam_reorder(cache, parents, length):
+        return cache
     if not cache.is_cuda:
         raise RuntimeError(f"beam_reorder: cache is on {cache.device}; asrq_b200 runs on CUDA (sm_100a) only and has no CPU path")
     _expect(cache.dim() == 5 and cache.is_contiguous() and parents.dim() == 2 and parents.numel() == cache.shape[1] and _ints(parents, cache),
@@ -91,6 +98,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     head_dim), ``k`` and ``v`` (B, S, key heads, head_dim), 16-bit, any strides with contiguous heads (``kv.view(B, S, 2, heads, head_dim)[:, :, i]`` of a
     fused projection); ``lengths`` (B,) int64 on the device, None for S everywhere.  ``scale`` head_dim ** -0.5 by default.  Returns (B, R, heads,
     head_dim); a row without keys is zero."""
+    if _linear._native is not None:
+        out = _linear._native.cross_attention(q, k, v, lengths, scale)
+        if out is not None:
+            return out
     dt = _require_cuda_16bit(q, "cross_attention")
     _expect(q.dim() == k.dim() == 4 and v.shape == k.shape, f"cross_attention: q (B, R, heads, head_dim), k and v (B, S, key heads, head_dim), got "
             f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -116,6 +127,10 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     prompt's keys and values once per utterance, (B, key heads, P, head_dim); each beam's own, (B * K, key heads, M, head_dim).  ``suffix_lengths``
     int64 on the device: one for all beams, or B * K; ``prefix_lengths`` (B,) int64, None for P everywhere.  Returns (B, K, heads, head_dim); a
     row without keys is zero."""
+    if _linear._native is not None:
+        out = _linear._native.prefix_attention(q, k_prefix, v_prefix, k_suffix, v_suffix, suffix_lengths, prefix_lengths, scale)
+        if out is not None:
+            return out
     dt = _require_cuda_16bit(q, "prefix_attention")
     _expect(q.dim() == k_prefix.dim() == k_suffix.dim() == 4 and v_prefix.shape == k_prefix.shape and v_suffix.shape == k_suffix.shape,
             "prefix_attention: q (B, K, heads, head_dim), prefix (B, key heads, P, head_dim), suffix (B * K, key heads, M, head_dim)")

@@ -6,23 +6,33 @@
 //   beam_reorder   cache[.., b * K + k, .., t] = cache[.., b * K + parent[b, k], .., t] for t < length, in place: bound by memory, the
 //                  rows that change written once and those they come from read once.
 //
-// The selection of an utterance is one cluster of 8 or 16 blocks and one launch, with no scratch in global memory, no counters
-// that outlive the launch and no order of arrival in the result.  A warp reads a segment of one beam's row, 2048 values at a time in
-// registers: their maximum and sum of exponentials, and the best n of the segment as a sorted list, one entry a lane.  Values enter
-// the list only past a threshold (the n-th largest of the lanes' maxima, the list's n-th entry), which a handful of 2048 pass.
-// A list entry is one word: the value as an ordered 16-bit number above the complement of its place in the segment, so that
-// equal values sort by their place.  The blocks of the cluster read each other's maxima, sums and list heads: every block then knows each beam's
-// normalisation (in 64 bits: the order of beams is decided by differences of sums) and the n-th best head, and sends what is no
-// worse than that, n * n entries at most, to the first block, which ranks it.
+// The selection of an utterance is one cluster of 4 to 16 blocks and one launch, with no scratch in global memory, no counters
+// that outlive the launch and no order of arrival in the result.  A warp reads a segment of one beam's row, 1024 values at a time:
+// each lane keeps the maximum and the sum of exponentials of its own values.  The warps of a block that share a row then agree on a value that
+// n of the lanes' maxima reach, and only the lanes whose maximum does (n of the row's lanes in the block, if maxima differ) are read again, by
+// the whole warp; what reaches it goes into the segment's list, of 32 entries at most, of which the best n are there.
+// An entry is one word: the value as an ordered 16-bit number above the complement of its place in the segment, so that
+// equal values sort by their place.  A row's segments do not depend on where it lies in memory, so beams with equal logits have equal
+// sums.  Maxima, sums and lists go to the first block of the cluster, which joins the sums in 64 bits (the order of beams is decided by their
+// differences) and ranks what is no worse than a bound that n of the lists' best reach.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
 #include "tcgen05.cuh"
 
 namespace asrq {
+
+int ensure_dynamic_smem(const void* kernel, size_t bytes);
+
 namespace {
 
-constexpr int kSelWarps = 8, kSelThreads = 32 * kSelWarps;
+constexpr int kSelWarps = 16, kSelThreads = 32 * kSelWarps;
 constexpr int kSelLists = 16 * kSelWarps;  // at most: one per warp of the cluster
 constexpr int kSelMax = 32;                // beams, and continuations asked for
-constexpr int kSelVecs = 8;                // 16-byte vectors a lane holds at a time
+constexpr int kSelVecs = 4;                // 16-byte vectors a lane holds at a time
+constexpr int kSelWords = 4 * kSelVecs;
+constexpr int kSelKept = 32 * kSelMax;     // candidates that are ranked: n lists of 32
 constexpr int kSegValues = 65536;          // places that a list entry tells apart (beam_select_fits)
 
 struct SelectParams {
@@ -38,7 +48,7 @@ struct SelectParams {
 
 struct __align__(16) ListMeta {  // what a warp knows of its segment
   double sum;      // of exp(x - top)
-  float top;       // NaN or +inf: the row is no distribution
+  float top;       // +inf: the row is no distribution
   uint32_t head;   // its best entry, 0: none
 };
 
@@ -128,217 +138,372 @@ __device__ __forceinline__ uint4 eight_of(const uint16_t* row, int e, int V, uin
 }
 
 // Candidates of an utterance: a larger key first, of equals the smaller place (beam * V + token)
-struct Cand {
+struct __align__(16) Cand {
   unsigned long long key;  // 0: none
-  uint32_t place;
+  uint32_t place, pad;
 };
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.key > b.key || (a.key == b.key && a.place < b.place); }
+__device__ __forceinline__ Cand ld_cand(const Cand* p) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  return Cand{(unsigned long long)u.x | ((unsigned long long)u.y << 32), u.z, 0};
+}
 
 enum RowState { kRowLive = 0, kRowOver = 1, kRowNone = 2 };
 
+constexpr float kLog2e = 1.4426950408889634f;
+struct F2 {  // two 32-bit numbers that one instruction works on
+  unsigned long long v;
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+
+// The n largest of a warp's words, two a lane, all different (or 0: none), descending over the lanes
+__device__ __forceinline__ uint32_t best_of(uint32_t a, uint32_t b, int n, int lane) {
+  if (n > 12) return merge_descending(sort_descending(a, lane), sort_descending(b, lane), lane);
+  uint32_t out = 0;
+  for (int i = 0; i < n; ++i) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, max(a, b));
+    if (a == m) a = 0;
+    if (b == m) b = 0;
+    if (lane == i) out = m;
+  }
+  return out;
+}
+
+struct SelectShared {  // of the first block, but for floors
+  uint32_t floors[kSelWarps][8];     // each block: a warp's largest lane maxima
+  uint8_t order[kSelWarps][32];      // each block: the lanes that a warp reads again
+  ListMeta meta[kSelLists];
+  uint32_t lists[kSelLists][kSelMax];
+  Cand heads[kSelLists + kSelMax];   // of the lists, and of the beams that do not go on
+  Cand kept[kSelKept];
+  double row_norm[kSelMax], row_score[kSelMax];
+  int row_state[kSelMax], live_row[kSelMax];
+  uint8_t row_over[kSelMax];
+  Cand bound;
+  uint32_t edge;
+  unsigned n_kept;
+  int n_live;
+};
+
 template <bool bf16>
-__global__ void __launch_bounds__(kSelThreads) beam_select_kernel(const SelectParams p) {
-  __shared__ ListMeta meta[kSelWarps];
-  __shared__ ListMeta all_meta[kSelLists];
-  __shared__ uint32_t lists[kSelWarps][32];
-  __shared__ Cand heads[kSelLists];
-  __shared__ double row_norm[kSelMax];
-  __shared__ double row_score[kSelMax];
-  __shared__ int row_state[kSelMax];
-  __shared__ Cand bound;
-  __shared__ unsigned kept;
-  __shared__ unsigned long long kept_key[kSelMax * kSelMax];
-  __shared__ uint32_t kept_place[kSelMax * kSelMax];
-  constexpr float kLog2e = 1.4426950408889634f;
+__global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const SelectParams p) {
+  extern __shared__ __align__(16) uint8_t select_smem[];
+  SelectShared& sh = *reinterpret_cast<SelectShared*>(select_smem);
   constexpr uint32_t kNone = bf16 ? 0xff80u : 0xfc00u;  // -inf
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank, blocks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+  // the first block's shared memory is written by the others once it is known to run: arrived here, waited for before the first write
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int b = int(blockIdx.x / blocks), n = p.n, K = p.K, V = p.V;
-  const int n_lists = int(blocks) * kSelWarps, per_row = n_lists / K;  // warps of a row
-  const int nvec = (V + 7) / 8, seg_vecs = (nvec + per_row - 1) / per_row;
-  const int id = int(rank) * kSelWarps + warp, row = id / per_row, seg = id - row * per_row;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const volatile float* scores = p.scores + size_t(b) * K;
   const volatile uint8_t* over = p.finished ? p.finished + size_t(b) * K : nullptr;
-  if (threadIdx.x == 0) kept = 0;
-  if (threadIdx.x < K) {
-    const float s = scores[threadIdx.x];
-    row_score[threadIdx.x] = double(s);
-    row_state[threadIdx.x] = !isfinite(s) ? kRowNone : over && over[threadIdx.x] ? kRowOver : kRowLive;
+  const int nvec = (V + 7) / 8, n_lists = int(blocks) * kSelWarps, id = int(rank) * kSelWarps + warp;
+  uint32_t y[kSelWords];  // the next values
+  auto load = [&](const uint16_t* r, int vb, int v1) {
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(r)) & 15u;
+    if (vb > 0 && vb + 32 * kSelVecs <= v1 && (vb + 32 * kSelVecs + 1) * 8 <= V) {  // all of it and its neighbours inside the row
+      const uint16_t* lo = r + size_t(vb + lane) * 8 - off / 2;
+      auto shifted = [&](auto words) {
+#pragma unroll
+        for (int i = 0; i < kSelVecs; ++i) {
+          const uint4 a0 = ld_x4(lo + i * 256), a1 = ld_x4(lo + i * 256 + 8);
+          const uint32_t w[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[4 * i + j] = __funnelshift_r(w[words.value + j], w[words.value + j + 1], (off & 2u) * 8u);
+        }
+      };
+      if (off == 0) {
+#pragma unroll
+        for (int i = 0; i < kSelVecs; ++i) {
+          const uint4 u = ld_x4(lo + i * 256);
+          y[4 * i] = u.x, y[4 * i + 1] = u.y, y[4 * i + 2] = u.z, y[4 * i + 3] = u.w;
+        }
+      } else if (off < 4) {
+        shifted(std::integral_constant<int, 0>{});
+      } else if (off < 8) {
+        shifted(std::integral_constant<int, 1>{});
+      } else if (off < 12) {
+        shifted(std::integral_constant<int, 2>{});
+      } else {
+        shifted(std::integral_constant<int, 3>{});
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kSelVecs; ++i) {
+      const int v = vb + i * 32 + lane;
+      const uint4 u = v < v1 ? eight_of(r, v * 8, V, kNone) : make_uint4(kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u);
+      y[4 * i] = u.x, y[4 * i + 1] = u.y, y[4 * i + 2] = u.z, y[4 * i + 3] = u.w;
+    }
+  };
+  const float early = warp == 0 && lane < K ? scores[lane] : 0.f;
+  const bool early_over = over && warp == 0 && lane < K && over[lane];
+  // most often all beams go on: the first values as if they did, while the scores are on their way
+  const int guess_per_row = n_lists / K, guess_row = id / guess_per_row;
+  if (guess_row < K) {
+    const int seg_vecs = (nvec + guess_per_row - 1) / guess_per_row, v0 = (id - guess_row * guess_per_row) * seg_vecs, v1 = min(nvec, v0 + seg_vecs);
+    if (v0 < v1) load(p.logits + size_t(b) * p.sb + size_t(guess_row) * p.sk, v0, v1);
+  }
+  if (warp == 0) {
+    int state = kRowNone;
+    if (lane < K) {
+      state = !isfinite(early) ? kRowNone : early_over ? kRowOver : kRowLive;
+      sh.row_score[lane] = double(early);
+      sh.row_state[lane] = state;
+      sh.row_over[lane] = early_over;
+    }
+    const unsigned live = __ballot_sync(0xffffffffu, state == kRowLive);
+    if (state == kRowLive) sh.live_row[__popc(live & ((1u << lane) - 1u))] = lane;
+    if (lane == 0) {
+      sh.n_live = __popc(live);
+      sh.n_kept = 0;
+    }
   }
   __syncthreads();
-
-  uint32_t list = 0;             // this lane's entry of the warp's list, descending over the lanes
-  float top = -INFINITY;         // of the warp's values so far
-  double sum = 0.0;              // of exp(x - top), this lane's
-  bool bad = false;
-  if (row < K && row_state[row] == kRowLive) {
-    const uint16_t* r = p.logits + size_t(b) * p.sb + size_t(row) * p.sk;
-    const int v0 = seg * seg_vecs, v1 = min(nvec, v0 + seg_vecs);
+  // the warps of the cluster share out the rows that go on
+  const int n_live = sh.n_live, per_row = n_lists / max(n_live, 1), seg_vecs = (nvec + per_row - 1) / per_row;
+  const int row_id = id / per_row, seg = id - row_id * per_row, v0 = seg * seg_vecs, v1 = min(nvec, v0 + seg_vecs);
+  const bool works = row_id < n_live && v0 < v1;
+  const uint16_t* r = works ? p.logits + size_t(b) * p.sb + size_t(sh.live_row[row_id]) * p.sk : nullptr;
+  float top = -INFINITY;       // of the warp's values
+  double sum = 0.0;            // of exp(x - top), this lane's
+  uint32_t mine = kNone * 0x10001u;  // this lane's maximum, of low and high halves
+  if (works) {
+    if (!(row_id == guess_row && n_live == K)) load(r, v0, v1);
 #pragma unroll 1
     for (int vb = v0; vb < v1; vb += 32 * kSelVecs) {
-      uint32_t x[kSelVecs][4];
+      uint32_t x[kSelWords], mx = y[0];
 #pragma unroll
-      for (int i = 0; i < kSelVecs; ++i) {
-        const int v = vb + i * 32 + lane;
-        const uint4 u = v < v1 ? eight_of(r, v * 8, V, kNone) : make_uint4(kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u);
-        x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
-      }
-      uint32_t mx = x[0][0];
+      for (int i = 0; i < kSelWords; ++i) x[i] = y[i];
 #pragma unroll
-      for (int i = 0; i < 4 * kSelVecs; ++i) mx = max2<bf16>(mx, x[i / 4][i % 4]);
-      const float lo = out16_to_float(uint16_t(mx & 0xffffu), bf16), hi = out16_to_float(uint16_t(mx >> 16), bf16);
-      bad |= !(fmaxf(lo, hi) < INFINITY) || lo != lo || hi != hi;
-      const uint32_t best = ordered16(lo >= hi ? mx & 0xffffu : mx >> 16);  // this lane's largest
-      const uint32_t by_lane = sort_descending(best, lane);
-      const uint32_t least = __shfl_sync(0xffffffffu, by_lane, n - 1);      // n values of the chunk are at least this
-      const float chunk_top = out16_to_float(unordered16(__shfl_sync(0xffffffffu, by_lane, 0)), bf16);
-      const float now = fmaxf(top, chunk_top), ref = now > -INFINITY ? now : 0.f;
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 1; i < kSelWords; ++i) mx = max2<bf16>(mx, x[i]);
+      if (vb + 32 * kSelVecs < v1) load(r, vb + 32 * kSelVecs, v1);
+      mine = max2<bf16>(mine, mx);
+      // (a NaN may pass as any maximum here: the row is no distribution then)
+      const float lane_top = fmaxf(out16_to_float(uint16_t(mine & 0xffffu), bf16), out16_to_float(uint16_t(mine >> 16), bf16)), ref = lane_top > -INFINITY ? lane_top : 0.f;
+      const F2 less(-ref, -ref), log2e(kLog2e, kLog2e);
+      F2 acc[2] = {F2(0.f, 0.f), F2(0.f, 0.f)};
 #pragma unroll
-      for (int i = 0; i < 4 * kSelVecs; ++i) {
-        const uint32_t w = x[i / 4][i % 4];
-        acc[i % 2] += exp2_fast((out16_to_float(uint16_t(w & 0xffffu), bf16) - ref) * kLog2e);
-        acc[2 + i % 2] += exp2_fast((out16_to_float(uint16_t(w >> 16), bf16) - ref) * kLog2e);
+      for (int i = 0; i < kSelWords; ++i) {
+        float d, e;
+        ((F2(out16_to_float(uint16_t(x[i] & 0xffffu), bf16), out16_to_float(uint16_t(x[i] >> 16), bf16)) + less) * log2e).get(d, e);
+        acc[i % 2] = acc[i % 2] + F2(exp2_fast(d), exp2_fast(e));
       }
-      sum = sum * double(top > -INFINITY ? exp2f((top - ref) * kLog2e) : 0.f) + double((acc[0] + acc[1]) + (acc[2] + acc[3]));
-      top = now;
-      // what may enter the list
-      const uint32_t floor16 = max(least, __shfl_sync(0xffffffffu, list, n - 1) >> 16);
-      const uint32_t least2 = uint32_t(unordered16(floor16)) * 0x10001u;
-      uint32_t hits[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 4 * kSelVecs; ++i) {
-        const uint32_t m = ge2<bf16>(x[i / 4][i % 4], least2);
-        hits[i / 16] |= ((m & 1u) | ((m >> 15) & 2u)) << (2 * (i % 16));
-      }
-      for (;;) {
-        const bool have = (hits[0] | hits[1]) != 0;
-        if (!__any_sync(0xffffffffu, have)) break;
-        uint32_t entry = 0;
-        if (have) {
-          const int half = hits[0] ? 0 : 1, bit = __ffs(hits[half]) - 1, at = half * 32 + bit;  // value `at` of the lane's 64
-          hits[half] &= hits[half] - 1;
-          const int place = ((vb - v0) + (at / 8) * 32 + lane) * 8 + at % 8, token = v0 * 8 + place;
-          if (token < V && place < (v1 - v0) * 8) entry = (ordered16(ld_x1(r + token)) << 16) | uint32_t(kSegValues - 1 - place);
-        }
-        const uint32_t last = __shfl_sync(0xffffffffu, list, n - 1);
-        if (entry <= last) entry = 0;
-        if (__any_sync(0xffffffffu, entry != 0)) list = merge_descending(list, sort_descending(entry, lane), lane);
-      }
+      float s0, s1;
+      (acc[0] + acc[1]).get(s0, s1);
+      sum = sum * double(exp2_fast((top - ref) * kLog2e)) + double(s0 + s1);
+      top = lane_top;
     }
   }
+  const float lo = out16_to_float(uint16_t(mine & 0xffffu), bf16), hi = out16_to_float(uint16_t(mine >> 16), bf16);
+  const bool bad = __any_sync(0xffffffffu, !(fmaxf(lo, hi) < INFINITY) || lo != lo || hi != hi);
+  const uint32_t best = ordered16(lo >= hi ? mine & 0xffffu : mine >> 16);  // this lane's largest
+  const uint32_t by_lane = sort_descending(best, lane);
+  {  // from the lanes' maxima to the warp's
+    const float all = out16_to_float(unordered16(__shfl_sync(0xffffffffu, by_lane, 0)), bf16);
+    if (top > -INFINITY) sum *= double(exp2_fast((top - all) * kLog2e));
+    top = bad ? INFINITY : all;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  bad = __any_sync(0xffffffffu, bad);
-  lists[warp][lane] = lane < n ? list : 0;
-  if (lane == 0) {
-    meta[warp].sum = sum;
-    meta[warp].top = bad ? INFINITY : top;
-    meta[warp].head = list;
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  tc::cluster_sync();
-  for (int i = threadIdx.x; i < n_lists; i += kSelThreads) {
-    const uint32_t at = tc::mapa(tc::smem_u32(&meta[i % kSelWarps]), uint32_t(i / kSelWarps));
-    const float4 m = tc::ld_dsmem_v4(at);
-    *reinterpret_cast<float4*>(&all_meta[i]) = m;
-  }
+  if (lane < 8) sh.floors[warp][lane] = by_lane;
   __syncthreads();
-  for (int k = warp; k < K; k += kSelWarps) {  // a beam's normalisation
-    if (row_state[k] != kRowLive) {
-      if (lane == 0) row_norm[k] = 0.0;
-      continue;
+  uint32_t list = 0;  // this lane's entry of the warp's list
+  if (works && !bad) {
+    uint32_t last = 0;  // n entries are no worse
+    // n values of the row are at least `least`: of this warp's lanes, or of the first few of each of the block's warps on this row
+    uint32_t least = __shfl_sync(0xffffffffu, by_lane, n - 1);
+    const int w0 = max(warp - seg, 0), w1 = min(warp + per_row - seg, kSelWarps), each = min(8, 32 / (w1 - w0));
+    if (each * (w1 - w0) >= n) {
+      const uint32_t at = lane < each * (w1 - w0) ? *(const volatile uint32_t*)&sh.floors[w0 + lane / each][lane % each] : 0u;
+      least = max(least, __shfl_sync(0xffffffffu, sort_descending(at, lane), n - 1));
     }
+    const uint32_t least2 = uint32_t(unordered16(least)) * 0x10001u;
+    int waiting = 0;  // entries so far, at most 32, in no order
+    volatile uint32_t* wait_at = sh.lists[warp];
+    const unsigned again = __ballot_sync(0xffffffffu, best >= least);
+    if (best >= least) sh.order[warp][__popc(again & ((1u << lane) - 1u))] = uint8_t(lane);
+    __syncwarp();
+    // every lane's values are `per` vectors; the warp takes 64 vectors of the chosen lanes at a time, the next ones on their way
+    const int per = (v1 - v0 + 31) / 32, items = __popc(again) * per;
+    int at_next[2];
+    uint4 next[2];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int item = i0 + 32 * h + lane, v = item < items ? v0 + sh.order[warp][item / per] + 32 * (item % per) : v1;
+        at_next[h] = v;
+        next[h] = v < v1 ? eight_of(r, v * 8, V, kNone) : make_uint4(kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u);
+      }
+    };
+    fetch(0);
+#pragma unroll 1
+    for (int i0 = 0; i0 < items; i0 += 64) {
+      const uint4 u0 = next[0], u1 = next[1];
+      const int v[2] = {at_next[0], at_next[1]};
+      if (i0 + 64 < items) fetch(i0 + 64);
+      const uint32_t w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+      uint32_t hits = 0;  // bit j: low half of word j, bit 16 + j: its high half
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hits |= ge2<bf16>(w[j], least2) & (0x10001u << j);
+      if (v[0] >= v1) hits &= 0xf0f0f0f0u;
+      if (v[1] >= v1) hits &= 0x0f0f0f0fu;
+      while (__any_sync(0xffffffffu, hits != 0)) {
+        uint32_t entry = 0;
+        if (hits) {
+          const int bit = __ffs(hits) - 1, j = bit & 15, place = ((j < 4 ? v[0] : v[1]) - v0) * 8 + 2 * (j & 3) + (bit >> 4);
+          hits &= hits - 1;
+          uint32_t word = w[0];
+#pragma unroll
+          for (int x = 1; x < 8; ++x)
+            if (j == x) word = w[x];
+          if (v0 * 8 + place < V) entry = (ordered16(bit >> 4 ? word >> 16 : word & 0xffffu) << 16) | uint32_t(kSegValues - 1 - place);
+        }
+        if (entry <= last) entry = 0;
+        const unsigned who = __ballot_sync(0xffffffffu, entry != 0);
+        if (waiting + __popc(who) > 32) {  // only the best n stay
+          __syncwarp();
+          const uint32_t now = best_of(lane < waiting ? wait_at[lane] : 0u, entry, n, lane);
+          __syncwarp();
+          wait_at[lane] = now;
+          waiting = n;
+          last = __shfl_sync(0xffffffffu, now, n - 1);
+          continue;
+        }
+        if (entry) wait_at[waiting + __popc(who & ((1u << lane) - 1u))] = entry;
+        waiting += __popc(who);
+      }
+    }
+    __syncwarp();
+    list = lane < waiting ? wait_at[lane] : 0u;
+  }
+  const uint32_t head = __reduce_max_sync(0xffffffffu, list);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::mapa(tc::smem_u32(&sh.lists[id][lane]), 0)), "r"(list) : "memory");
+  if (lane == 0)
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(tc::mapa(tc::smem_u32(&sh.meta[id]), 0)), "r"(uint32_t(__double2loint(sum))),
+                 "r"(uint32_t(__double2hiint(sum))), "r"(__float_as_uint(top)), "r"(head)
+                 : "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (rank != 0) return;
+  for (int i = warp; i < n_live; i += kSelWarps) {  // a beam's normalisation
+    const int k = sh.live_row[i];
+    const ListMeta* of = sh.meta + i * per_row;
     float t = -INFINITY;
-    for (int i = lane; i < per_row; i += 32) t = fmaxf(t, all_meta[k * per_row + i].top);
+    for (int j = lane; j < per_row; j += 32) t = fmaxf(t, of[j].top);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+    if (!isfinite(t)) {
+      if (lane == 0) sh.row_state[k] = kRowNone;
+      continue;
+    }
     double s = 0.0;
-    if (isfinite(t))
-      for (int i = lane; i < per_row; i += 32) {
-        const ListMeta& m = all_meta[k * per_row + i];
-        if (m.top > -INFINITY) s += m.sum * exp(double(m.top) - double(t));
-      }
+    for (int j = lane; j < per_row; j += 32) s += of[j].sum * double(exp2_fast((of[j].top - t) * kLog2e));
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) {
-      row_norm[k] = double(t) + log(s);
-      if (!isfinite(t)) row_state[k] = kRowNone;
-    }
+    if (lane == 0) sh.row_norm[k] = double(t) + log(s);
   }
   __syncthreads();
-  // entry `at` of list `l`; `word`: what the list holds there
-  auto candidate = [&](int l, int at, uint32_t word) {
-    const int k = l / per_row, sg = l - k * per_row;
-    Cand c = {0, 0};
-    if (k >= K) return c;
-    const int state = row_state[k];
-    if (state == kRowLive) {
-      if (!word) return c;
-      const uint32_t token = uint32_t(sg) * uint32_t(seg_vecs) * 8u + (kSegValues - 1 - (word & 0xffffu));
-      const float x = out16_to_float(unordered16(word >> 16), bf16);
-      c.key = ordered64(x > -INFINITY ? row_score[k] + (double(x) - row_norm[k]) : -INFINITY);
-      c.place = uint32_t(k) * uint32_t(V) + token;
-      return c;
-    }
-    // an ended beam: the end token at its own score, then the lowest others; a beam without hypothesis: the lowest tokens
-    if (sg != 0 || at >= min(n, V)) return c;
+  auto of_list = [&](int l, uint32_t word) {  // an entry of list l
+    const int i = l / per_row;
+    Cand q = {0, 0, 0};
+    if (i >= n_live || !word) return q;
+    const int k = sh.live_row[i];
+    if (sh.row_state[k] != kRowLive) return q;
+    const uint32_t token = uint32_t(l - i * per_row) * uint32_t(seg_vecs) * 8u + (kSegValues - 1 - (word & 0xffffu));
+    const float v = out16_to_float(unordered16(word >> 16), bf16);
+    q.key = ordered64(v > -INFINITY ? sh.row_score[k] + (double(v) - sh.row_norm[k]) : -INFINITY);
+    q.place = uint32_t(k) * uint32_t(V) + token;
+    return q;
+  };
+  auto of_beam = [&](int k, int at) {  // an ended beam: the end token at its own score, then the lowest others; one without hypothesis: the lowest tokens
+    Cand q = {0, 0, 0};
+    if (k >= K || sh.row_state[k] == kRowLive || at >= min(n, V)) return q;
     int token = at;
     double s = -INFINITY;
-    if (state == kRowOver) {
-      if (at == 0) s = row_score[k];
+    if (sh.row_state[k] == kRowOver) {
+      if (at == 0) s = sh.row_score[k];
       token = at == 0 ? p.eos : at - 1 < p.eos ? at - 1 : at;
     }
-    c.key = ordered64(s);
-    c.place = uint32_t(k) * uint32_t(V) + uint32_t(token);
-    return c;
+    q.key = ordered64(s);
+    q.place = uint32_t(k) * uint32_t(V) + uint32_t(token);
+    return q;
   };
-  if (threadIdx.x == 0) bound = Cand{0, 0xffffffffu};
-  for (int l = threadIdx.x; l < n_lists; l += kSelThreads) heads[l] = candidate(l, 0, all_meta[l].head);
+  // The heads, one a thread: of the lists, then of the beams that do not go on; neighbours to different warps.
+  const int n_heads = n_lists + kSelMax, head_at = lane * kSelWarps + warp;
+  const Cand head_cand = head_at < n_lists ? of_list(head_at, sh.meta[head_at].head) : of_beam(head_at - n_lists, 0);
+  if (head_at < n_heads) sh.heads[head_at] = head_cand;
   __syncthreads();
-  for (int l = threadIdx.x; l < n_lists; l += kSelThreads) {
-    const Cand c = heads[l];
-    if (!c.key) continue;
-    int ahead = 0;
-    for (int i = 0; i < n_lists; ++i) ahead += before(heads[i], c);
-    if (ahead == n - 1) bound = c;  // one at most: no two candidates share a place
+  if (warp == 0) {  // the n-th largest of 32 lanes' maxima of heads: n candidates are no worse, by the high words alone
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < kSelLists / 32 + 1; ++j)
+      if (j * 32 < n_heads) most = max(most, uint32_t(sh.heads[j * 32 + lane].key >> 32));
+    const uint32_t nth = __shfl_sync(0xffffffffu, sort_descending(most, lane), n - 1);
+    if (lane == 0) sh.edge = nth;
   }
   __syncthreads();
-  {
-    const Cand c = lane < n ? candidate(id, lane, lists[warp][lane]) : Cand{0, 0};
-    const bool keep = c.key && !before(bound, c);
-    const unsigned who = __ballot_sync(0xffffffffu, keep);
-    if (who) {
+  const uint32_t edge = sh.edge;
+  Cand bound = {0, 0, 0};  // with a key: as well as the edge
+  auto gather = [&]() {
+    auto passes = [&](const Cand& q) { return q.key && uint32_t(q.key >> 32) >= edge && !(bound.key && before(bound, q)); };
+    for (unsigned todo = __ballot_sync(0xffffffffu, head_at < n_heads && passes(head_cand)); todo; todo &= todo - 1) {
+      const int l = (__ffs(todo) - 1) * kSelWarps + warp;
+      const Cand q = l < n_lists ? of_list(l, sh.lists[l][lane]) : of_beam(l - n_lists, lane);
+      const bool keep = passes(q);
+      const unsigned who = __ballot_sync(0xffffffffu, keep);
       unsigned first = 0;
-      if (lane == 0) {
-        const uint32_t at = tc::mapa(tc::smem_u32(&kept), 0);
-        asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(first) : "r"(at), "r"(unsigned(__popc(who))) : "memory");
-      }
+      if (lane == 0) first = atomicAdd(&sh.n_kept, unsigned(__popc(who)));
       first = __shfl_sync(0xffffffffu, first, 0) + __popc(who & ((1u << lane) - 1u));
-      if (keep && first < kSelMax * kSelMax) {
-        const uint32_t kat = tc::mapa(tc::smem_u32(&kept_key[first]), 0), pat = tc::mapa(tc::smem_u32(&kept_place[first]), 0);
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(kat), "l"(c.key) : "memory");
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(pat), "r"(c.place) : "memory");
-      }
+      if (keep && first < kSelKept) sh.kept[first] = q;
     }
+    __syncthreads();
+  };
+  gather();
+  if (sh.n_kept > kSelKept) {
+    // Equal high words beyond number: the n-th best head itself, which leaves n lists.
+    if (head_at < n_heads && head_cand.key) {
+      int ahead = 0;
+      for (int j = 0; j < n_heads; ++j) ahead += before(ld_cand(&sh.heads[j]), head_cand);
+      if (ahead == n - 1) sh.bound = head_cand;  // there is one: more than n heads pass, and no two share a place
+    }
+    __syncthreads();
+    bound = ld_cand(&sh.bound);
+    if (threadIdx.x == 0) sh.n_kept = 0;
+    __syncthreads();
+    gather();
   }
-  tc::cluster_sync();
-  if (rank != 0) return;
-  const int m = int(min(kept, unsigned(kSelMax * kSelMax)));
-  for (int i = threadIdx.x; i < m; i += kSelThreads) {
-    const Cand c = {kept_key[i], kept_place[i]};
+  // the n best, in order: eight lanes count what is ahead of a candidate
+  const int m = int(min(sh.n_kept, unsigned(kSelKept))), part = lane & 7;
+  for (int i0 = warp * 4; i0 < m; i0 += kSelThreads / 8) {
+    const int i = i0 + lane / 8;
+    const Cand q = i < m ? ld_cand(&sh.kept[i]) : Cand{0, 0, 0};
     int ahead = 0;
-    for (int j = 0; j < m; ++j) ahead += before(Cand{kept_key[j], kept_place[j]}, c);
-    if (ahead >= n) continue;
+#pragma unroll 2
+    for (int j = part; j < m; j += 8) ahead += before(ld_cand(&sh.kept[j]), q);
+#pragma unroll
+    for (int x = 1; x < 8; x *= 2) ahead += __shfl_xor_sync(0xffffffffu, ahead, x);
+    if (i >= m || ahead >= n || part != 0) continue;
     const size_t o = size_t(b) * n + ahead;
-    const int k = int(c.place / uint32_t(V)), token = int(c.place - uint32_t(k) * uint32_t(V));
-    p.out_scores[o] = float(unordered64(c.key));
+    const int k = int(q.place / uint32_t(V)), token = int(q.place - uint32_t(k) * uint32_t(V));
+    p.out_scores[o] = float(unordered64(q.key));
     p.parents[o] = k;
     p.tokens[o] = token;
-    if (over) p.out_finished[o] = over[k] || token == p.eos;
+    if (over) p.out_finished[o] = sh.row_over[k] || token == p.eos;
   }
 }
 
@@ -381,9 +546,36 @@ beam_reorder_kernel(uint4* __restrict__ cache, const long long* parents, const l
 
 }  // namespace
 
-bool beam_select_fits(int64_t K, int64_t V) {
-  const int64_t per_row = kSelLists / K;  // sixteen blocks
-  return ((V + 7) / 8 + per_row - 1) / per_row * 8 <= kSegValues;
+// whether the segments of a cluster of `blocks` are short enough for their lists
+bool segments_fit(int64_t blocks, int64_t K, int64_t V) {
+  const int64_t per_row = blocks * kSelWarps / K;
+  return per_row > 0 && ((V + 7) / 8 + per_row - 1) / per_row * 8 <= kSegValues;
+}
+bool beam_select_fits(int64_t K, int64_t V) { return segments_fit(8, K, V); }
+
+// clusters of `blocks` that the chip holds at once
+int64_t select_clusters(int blocks, int sm_count) {
+  static std::atomic<int> known[17];  // one kind of device: asked once per process
+  int n = known[blocks].load(std::memory_order_relaxed);
+  if (n) return n;
+  cudaFuncSetAttribute(beam_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SelectShared)));
+  cudaFuncSetAttribute(beam_select_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = sizeof(SelectShared);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(blocks);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, beam_select_kernel<false>, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = std::max(1, sm_count / blocks);
+  }
+  known[blocks].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores, const uint8_t* finished, int64_t eos, float* out_scores,
@@ -403,18 +595,21 @@ int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores,
   p.V = int(V);
   p.n = int(n);
   p.eos = int(eos);
-  // sixteen blocks an utterance while eight would leave half of the chip idle, or where a segment of eight would be too long
-  const int64_t per_row8 = 8 * kSelWarps / K;
-  const bool wide = B * 16 <= sm_count || ((V + 7) / 8 + per_row8 - 1) / per_row8 * 8 > kSegValues;
   auto kern = dtype == ASRQ_BF16 ? beam_select_kernel<true> : beam_select_kernel<false>;
-  if (wide) ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), sizeof(SelectShared));
+  if (rc) return rc;
+  // As many blocks an utterance as the chip holds at once (64 utterances of 8 x 51866, us: 16 blocks @16, 8 @8, 4 @4).
+  int blocks = 16;
+  while (blocks > 4 && B > select_clusters(blocks, sm_count) && segments_fit(blocks / 2, K, V)) blocks /= 2;
+  if (blocks > 8) ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(B * (wide ? 16 : 8)));
+  cfg.gridDim = dim3(unsigned(B * blocks));
   cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = sizeof(SelectShared);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = wide ? 16 : 8;
+  attr[0].val.clusterDim.x = unsigned(blocks);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;

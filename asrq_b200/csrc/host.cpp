@@ -26,6 +26,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <atomic>
+#include <cmath>
 #include <map>
 #include <mutex>
 
@@ -311,6 +312,179 @@ PyObject* linearqq_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- decoding with beams: the calls of asrq_b200/beam.py, whose arguments the caller holds -------------------------------------------
+
+// A tensor of `type` on `dev` with `dims` dimensions, or None for an empty pointer.  False: not the ordinary case.
+bool operand(PyObject* o, const c10::Device& dev, at::ScalarType type, int64_t dims, bool contiguous, const at::Tensor** out) {
+  const at::Tensor* t = plain(o);
+  if (!t || t->device() != dev || t->scalar_type() != type || t->dim() != dims || (contiguous && !t->is_contiguous())) return false;
+  *out = t;
+  return true;
+}
+// The first operand: 16-bit on the current CUDA device
+const at::Tensor* leading(PyObject* o, int64_t dims, int* dtype) {
+  const at::Tensor* t = plain(o);
+  if (!t || !t->is_cuda() || t->dim() != dims || t->numel() == 0) return nullptr;
+  const auto st = t->scalar_type();
+  if (st != at::kHalf && st != at::kBFloat16) return nullptr;
+  *dtype = st == at::kHalf ? ASRQ_F16 : ASRQ_BF16;
+  return t->device().index() == c10::cuda::current_device() && !modes_active() ? t : nullptr;
+}
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const c10::Device& dev) { return at::detail::empty_cuda(shape, type, dev, std::nullopt); }
+
+// beam_select(logits, scores, n, finished or None, eos or None) -> tuple, or None: not the ordinary case
+PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  int dtype;
+  const at::Tensor *x, *s, *f = nullptr;
+  if (n_args != 5 || !(x = leading(a[0], 3, &dtype)) || (x->stride(2) != 1 && x->size(2) != 1) || !operand(a[1], x->device(), at::kFloat, 2, true, &s) ||
+      s->size(0) != x->size(0) || s->size(1) != x->size(1) || !PyLong_Check(a[2]) || (a[3] == Py_None) != (a[4] == Py_None))
+    Py_RETURN_NONE;
+  long long eos = 0;
+  if (a[3] != Py_None) {
+    if (!operand(a[3], x->device(), at::kBool, 2, true, &f) || f->sizes() != s->sizes() || !PyLong_Check(a[4])) Py_RETURN_NONE;
+    eos = PyLong_AsLongLong(a[4]);
+  }
+  const long long n = PyLong_AsLongLong(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (n <= 0 || n > 32) Py_RETURN_NONE;
+  const int64_t B = x->size(0);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  at::Tensor out[4];
+  int rc;
+  {
+    Unlocked unlocked;
+    out[0] = fresh({B, n}, at::kFloat, x->device());
+    out[1] = fresh({B, n}, at::kLong, x->device());
+    out[2] = fresh({B, n}, at::kLong, x->device());
+    if (f) out[3] = fresh({B, n}, at::kBool, x->device());
+    g_calls.fetch_add(1, std::memory_order_relaxed);
+    rc = asrq_beam_select(x->data_ptr(), x->stride(0), x->stride(1), static_cast<const float*>(s->data_ptr()), f ? static_cast<const uint8_t*>(f->data_ptr()) : nullptr,
+                          eos, static_cast<float*>(out[0].data_ptr()), static_cast<int64_t*>(out[1].data_ptr()), static_cast<int64_t*>(out[2].data_ptr()),
+                          f ? static_cast<uint8_t*>(out[3].data_ptr()) : nullptr, B, x->size(1), x->size(2), n, dtype, stream);
+  }
+  if (rc) return failed("asrq_beam_select", rc);
+  PyObject* tuple = PyTuple_New(f ? 4 : 3);
+  if (!tuple) return nullptr;
+  for (int i = 0; i < (f ? 4 : 3); ++i) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(out[i])));
+  return tuple;
+  END_HANDLE_TH_ERRORS
+}
+
+// beam_reorder(cache, parents, length tensor or int) -> True, or None
+PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *x = n_args == 3 ? plain(a[0]) : nullptr, *p, *len = nullptr;
+  if (!x || !x->is_cuda() || x->dim() != 5 || x->numel() == 0 || !x->is_contiguous() || x->device().index() != c10::cuda::current_device() || modes_active() ||
+      !operand(a[1], x->device(), at::kLong, 2, true, &p) || p->numel() != x->size(1))
+    Py_RETURN_NONE;
+  long long length = 0;
+  if (PyLong_Check(a[2])) {
+    length = PyLong_AsLongLong(a[2]);
+    if (PyErr_Occurred()) return nullptr;
+  } else {
+    len = plain(a[2]);
+    if (!len || len->device() != x->device() || len->scalar_type() != at::kLong || len->numel() != 1) Py_RETURN_NONE;
+  }
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  int rc;
+  {
+    Unlocked unlocked;
+    g_calls.fetch_add(1, std::memory_order_relaxed);
+    rc = asrq_beam_reorder(x->data_ptr(), static_cast<const int64_t*>(p->data_ptr()), len ? static_cast<const int64_t*>(len->data_ptr()) : nullptr, length, x->size(0),
+                           p->size(0), p->size(1), x->size(2), x->size(3), x->size(4) * x->element_size(), stream);
+  }
+  if (rc) return failed("asrq_beam_reorder", rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// The strides of three dimensions as the attention kernels take them.  False: they cannot read it as it is.
+bool strides_of(const at::Tensor& t, int d0, int d1, int d2, int64_t (&s)[3]) {
+  if (t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  const int d[3] = {d0, d1, d2};
+  for (int i = 0; i < 3; ++i) {
+    s[i] = t.size(d[i]) > 1 ? t.stride(d[i]) : 0;
+    if (s[i] % 8) return false;
+  }
+  return true;
+}
+// None, or int64 values on the device: `n` of them, or one where that may be
+bool lengths_of(PyObject* o, const c10::Device& dev, int64_t n, bool one, const at::Tensor** t) {
+  *t = nullptr;
+  if (o == Py_None) return true;
+  *t = plain(o);
+  return *t && (*t)->device() == dev && (*t)->scalar_type() == at::kLong && (*t)->is_contiguous() &&
+         ((*t)->numel() == n || (one && (*t)->numel() == 1)) && (one || (*t)->dim() == 1);
+}
+bool scale_of(PyObject* o, int64_t hd, float* scale) {
+  if (o == Py_None) {
+    *scale = float(1.0 / std::sqrt(double(hd)));
+    return true;
+  }
+  if (!PyFloat_Check(o)) return false;
+  *scale = float(PyFloat_AS_DOUBLE(o));
+  return true;
+}
+inline const int64_t* ints(const at::Tensor* t) { return t ? static_cast<const int64_t*>(t->data_ptr()) : nullptr; }
+
+// cross_attention(q, k, v, lengths or None, scale or None) -> out, or None
+PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  int dtype;
+  float scale;
+  const at::Tensor *q, *k, *v, *len;
+  int64_t qs[3], ks[3], vs[3];
+  if (n_args != 5 || !(q = leading(a[0], 4, &dtype)) || !operand(a[1], q->device(), q->scalar_type(), 4, false, &k) ||
+      !operand(a[2], q->device(), q->scalar_type(), 4, false, &v) || k->sizes() != v->sizes() || k->size(0) != q->size(0) || k->size(3) != q->size(3) ||
+      k->size(2) <= 0 || q->size(2) % k->size(2) || !lengths_of(a[3], q->device(), q->size(0), false, &len) || !scale_of(a[4], q->size(3), &scale) ||
+      !strides_of(*q, 0, 1, 2, qs) || !strides_of(*k, 0, 2, 1, ks) || !strides_of(*v, 0, 2, 1, vs))
+    Py_RETURN_NONE;
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(q->device().index()).stream();
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    out = fresh(q->sizes(), q->scalar_type(), q->device());
+    g_calls.fetch_add(1, std::memory_order_relaxed);
+    rc = asrq_cross_attention(q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, ints(len), out.data_ptr(), q->size(0), q->size(1), int(q->size(2)),
+                              int(k->size(2)), int(q->size(3)), k->size(1), scale, dtype, stream);
+  }
+  if (rc) return failed("asrq_cross_attention", rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// prefix_attention(q, k_prefix, v_prefix, k_suffix, v_suffix, suffix_lengths, prefix_lengths or None, scale or None) -> out, or None
+PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  int dtype;
+  float scale;
+  const at::Tensor *q, *kv[4], *own, *len;
+  int64_t qs[3], s[4][3];
+  if (n_args != 8 || !(q = leading(a[0], 4, &dtype))) Py_RETURN_NONE;
+  for (int i = 0; i < 4; ++i)
+    if (!operand(a[1 + i], q->device(), q->scalar_type(), 4, false, &kv[i]) || !strides_of(*kv[i], 0, 1, 2, s[i])) Py_RETURN_NONE;
+  const int64_t B = q->size(0), K = q->size(1), hkv = kv[0]->size(1), hd = q->size(3);
+  if (kv[0]->sizes() != kv[1]->sizes() || kv[2]->sizes() != kv[3]->sizes() || kv[0]->size(0) != B || kv[2]->size(0) != B * K || hkv <= 0 || q->size(2) % hkv ||
+      kv[2]->size(1) != hkv || kv[0]->size(3) != hd || kv[2]->size(3) != hd || a[5] == Py_None || !lengths_of(a[5], q->device(), B * K, true, &own) ||
+      !lengths_of(a[6], q->device(), B, false, &len) || !scale_of(a[7], hd, &scale) || !strides_of(*q, 0, 1, 2, qs))
+    Py_RETURN_NONE;
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(q->device().index()).stream();
+  at::Tensor out;
+  int rc;
+  {
+    Unlocked unlocked;
+    out = fresh(q->sizes(), q->scalar_type(), q->device());
+    g_calls.fetch_add(1, std::memory_order_relaxed);
+    rc = asrq_prefix_attention(q->data_ptr(), qs, kv[0]->data_ptr(), s[0], kv[1]->data_ptr(), s[1], ints(len), kv[2]->data_ptr(), s[2], kv[3]->data_ptr(), s[3],
+                               ints(own), own->numel(), out.data_ptr(), B, K, int(q->size(2)), int(hkv), int(hd), kv[0]->size(2), kv[2]->size(2), scale, dtype, stream);
+  }
+  if (rc) return failed("asrq_prefix_attention", rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* calls(PyObject*, PyObject*) { return PyLong_FromLongLong(g_calls.load(std::memory_order_relaxed)); }
 
 // A stream of this file's own per device: never under capture, which one of the pool that torch hands out round and round may be.
@@ -365,6 +539,10 @@ PyObject* bind(PyObject*, PyObject* args) {
 PyMethodDef kMethods[] = {
     {"linearq_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linearq_forward)), METH_FASTCALL, nullptr},
     {"linearqq_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linearqq_forward)), METH_FASTCALL, nullptr},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, nullptr},
+    {"beam_reorder", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_reorder)), METH_FASTCALL, nullptr},
+    {"cross_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cross_attention)), METH_FASTCALL, nullptr},
+    {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefix_attention)), METH_FASTCALL, nullptr},
     {"calls", calls, METH_NOARGS, nullptr},
     {"zeros_now", zeros_now, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},

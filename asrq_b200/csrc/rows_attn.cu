@@ -21,6 +21,9 @@
 #include "tcgen05.cuh"
 
 namespace asrq {
+
+int ensure_dynamic_smem(const void* kernel, size_t bytes);
+
 namespace {
 
 constexpr int kRowsWarps = 8;
@@ -354,7 +357,8 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
   p.tiles = (p.R * p.G + ROWS - 1) / ROWS;
   const int64_t items = B * p.Hkv * p.tiles;
   auto kern = rows_attn_kernel<HD, MT, BF16>;
-  ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+  if (rc) return rc;
   // blocks an item: until the chip is full, or a warp has a single chunk
   const int64_t chunks = (p.keys + KC - 1) / KC + (p.k2 ? (p.keys2 + KC - 1) / KC : 0);
   int split = 1;
