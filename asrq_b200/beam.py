@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from . import linear as _linear
-from .linear import _expect, _on_device, _require_cuda_16bit
+from .linear import _expect, _on_device, _require_cuda_16bit, _workspace
 
 
 def _ints(t: torch.Tensor, like: torch.Tensor) -> bool:
@@ -93,6 +93,14 @@ def _strides(x: torch.Tensor, *dims: int):
     return (ctypes.c_int64 * 3)(*(x.stride(d) if x.shape[d] > 1 else 0 for d in dims))
 
 
+def _memory(q: torch.Tensor, key_heads: int, shared: int, own: int):
+    """(workspace, its bytes, scratch, its bytes) of a call."""
+    ws = _workspace(q.device, _lib.STATUS_BYTES)
+    need = int(_lib.load().asrq_rows_attention_scratch_bytes(q.shape[0], q.shape[1], q.shape[2], key_heads, q.shape[3], shared, own))
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    return ws, ws.data_ptr(), ws.numel(), scratch, None if scratch is None else scratch.data_ptr(), need
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor = None, scale: float = None) -> torch.Tensor:
     """Attention of the rows of an utterance (the beams of a step, or the tokens of a prompt) over its encoder states: ``q`` (B, R, heads,
     head_dim), ``k`` and ``v`` (B, S, key heads, head_dim), 16-bit, any strides with contiguous heads (``kv.view(B, S, 2, heads, head_dim)[:, :, i]`` of a
@@ -115,9 +123,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: 
     out = torch.empty((B, R, Hq, hd), dtype=q.dtype, device=q.device)
     if out.numel():
         with _on_device(q.device):
+            ws, ws_ptr, ws_bytes, scratch, scratch_ptr, need = _memory(q, Hkv, S, 0)
             _lib.call("asrq_cross_attention", q.data_ptr(), _strides(q, 0, 1, 2), k.data_ptr(), _strides(k, 0, 2, 1), v.data_ptr(), _strides(v, 0, 2, 1),
                       None if lengths is None else lengths.data_ptr(), out.data_ptr(), B, R, Hq, Hkv, hd, S, hd ** -0.5 if scale is None else float(scale),
-                      dt, torch.cuda.current_stream(q.device).cuda_stream)
+                      dt, ws_ptr, ws_bytes, scratch_ptr, need, torch.cuda.current_stream(q.device).cuda_stream)
     return out
 
 
@@ -148,10 +157,12 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     out = torch.empty((B, K, Hq, hd), dtype=q.dtype, device=q.device)
     if out.numel():
         with _on_device(q.device):
+            ws, ws_ptr, ws_bytes, scratch, scratch_ptr, need = _memory(q, Hkv, P, M)
             _lib.call("asrq_prefix_attention", q.data_ptr(), _strides(q, 0, 1, 2), k_prefix.data_ptr(), _strides(k_prefix, 0, 1, 2), v_prefix.data_ptr(),
                       _strides(v_prefix, 0, 1, 2), None if prefix_lengths is None else prefix_lengths.data_ptr(), k_suffix.data_ptr(), _strides(k_suffix, 0, 1, 2),
                       v_suffix.data_ptr(), _strides(v_suffix, 0, 1, 2), suffix_lengths.data_ptr(), suffix_lengths.numel(), out.data_ptr(), B, K, Hq, Hkv, hd, P, M,
-                      hd ** -0.5 if scale is None else float(scale), dt, torch.cuda.current_stream(q.device).cuda_stream)
+                      hd ** -0.5 if scale is None else float(scale), dt, ws_ptr, ws_bytes, scratch_ptr, need,
+                      torch.cuda.current_stream(q.device).cuda_stream)
     return out
 
 

@@ -65,8 +65,9 @@ int beam_reorder(void* cache, const long long* parents, const long long* length_
                  int64_t max_len, int64_t pos_bytes, cudaStream_t stream);
 int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
                    const void* k2, const int64_t* k2s, const void* v2, const int64_t* v2s, const long long* lengths2, bool lengths2_many, void* out,
-                   int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, float scale, int dtype, int sm_count,
-                   cudaStream_t stream);
+                   int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, float scale, int dtype, void* status, void* scratch,
+                   size_t scratch_bytes, int sm_count, cudaStream_t stream);
+size_t rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count);
 int hadamard_quant_int4(const void* x, uint8_t* qa, float* sa, int64_t M, int64_t K, int hadamard, int dtype,
                         int out_int8, cudaStream_t stream);
 int w4a4_linear_tc(const void* x, const uint8_t* qw, const void* sw, const void* bias, void* y, int64_t M, int64_t N,
@@ -253,6 +254,19 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, bool bf16, 
   e.key = key;
   e.map = *out;
   e.used = true;
+  return ASRQ_OK;
+}
+
+int make_tmap_4d(CUtensorMap* out, const void* base, bool bf16, uint64_t inner, uint64_t d1, uint64_t d2, uint64_t d3, int64_t s1, int64_t s2, int64_t s3,
+                 uint32_t box_inner, uint32_t box_1) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(ASRQ_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
+  auto bytes = [&](uint64_t d, int64_t s) { return d > 1 ? cuuint64_t(s) * 2 : cuuint64_t(inner) * 2; };
+  const cuuint64_t dims[4] = {inner, d1, d2, d3}, strides[3] = {bytes(d1, s1), bytes(d2, s2), bytes(d3, s3)};
+  const cuuint32_t box[4] = {box_inner, box_1, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ASRQ_ERR_SHAPE, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
   return ASRQ_OK;
 }
 
@@ -765,7 +779,7 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
 namespace {
 // What the two attentions of shared keys have in common
 int check_rows(const char* who, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* out, int64_t B,
-               int64_t R, int nq, int nkv, int hd, int64_t keys, int dtype) {
+               int64_t R, int nq, int nkv, int hd, int64_t keys, int dtype, const void* scratch) {
   if (!q || !out || !qs || !ks || !vs || (keys > 0 && (!k || !v))) return fail(ASRQ_ERR_NULL, "%s: q, k, v, out and the strides must not be NULL", who);
   if (dtype != ASRQ_F16 && dtype != ASRQ_BF16) return fail(ASRQ_ERR_DTYPE, "%s: dtype %d", who, dtype);
   if (B < 0 || R < 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq > (1 << 16) || (hd != 64 && hd != 128) || keys < 0 || keys > 0x7fffffff || R > (1 << 24) ||
@@ -774,6 +788,7 @@ int check_rows(const char* who, const void* q, const int64_t* qs, const void* k,
   for (const int64_t* s : {qs, ks, vs})
     if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[0] % 8 || s[1] % 8 || s[2] % 8)
       return fail(ASRQ_ERR_ALIGN, "%s: strides %lld, %lld, %lld (multiples of 8)", who, (long long)s[0], (long long)s[1], (long long)s[2]);
+  if (scratch && !aligned16(scratch)) return fail(ASRQ_ERR_ALIGN, "%s: scratch must be 16-byte aligned", who);
   for (const void* x : {q, keys > 0 ? k : q, keys > 0 ? v : q})
     if (!aligned16(x)) return fail(ASRQ_ERR_ALIGN, "%s: q, k and v must be 16-byte aligned", who);
   return ASRQ_OK;
@@ -782,28 +797,29 @@ int check_rows(const char* who, const void* q, const int64_t* qs, const void* k,
 
 int asrq_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                          const int64_t* lengths, void* out, int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t keys, float scale,
-                         int dtype, void* stream) {
+                         int dtype, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
   last_error().clear();
-  int rc = check_rows("asrq_cross_attention", q, q_strides, k, k_strides, v, v_strides, out, B, R, n_q_heads, n_kv_heads, head_dim, keys, dtype);
+  int rc = check_rows("asrq_cross_attention", q, q_strides, k, k_strides, v, v_strides, out, B, R, n_q_heads, n_kv_heads, head_dim, keys, dtype, scratch);
   if (rc) return rc;
   const DeviceFacts* f;
   if ((rc = device_facts(&f))) return rc;
   if (B == 0 || R == 0) return ASRQ_OK;
   return rows_attention(q, q_strides, k, k_strides, v, v_strides, reinterpret_cast<const long long*>(lengths), nullptr, nullptr, nullptr, nullptr, nullptr, false, out,
-                        B, R, n_q_heads, n_kv_heads, head_dim, keys, 0, scale, dtype, f->sm_count, static_cast<cudaStream_t>(stream));
+                        B, R, n_q_heads, n_kv_heads, head_dim, keys, 0, scale, dtype, workspace_bytes >= kStatusBytes ? workspace : nullptr, scratch, scratch_bytes, f->sm_count,
+                        static_cast<cudaStream_t>(stream));
 }
 
 int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k_prefix, const int64_t* k_prefix_strides, const void* v_prefix,
                           const int64_t* v_prefix_strides, const int64_t* prefix_lengths, const void* k_suffix, const int64_t* k_suffix_strides,
                           const void* v_suffix, const int64_t* v_suffix_strides, const int64_t* suffix_lengths, int64_t n_suffix_lengths, void* out, int64_t B,
                           int64_t K, int n_q_heads, int n_kv_heads, int head_dim, int64_t prefix_keys, int64_t suffix_keys, float scale, int dtype,
-                          void* stream) {
+                          void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
   last_error().clear();
   int rc = check_rows("asrq_prefix_attention", q, q_strides, k_prefix, k_prefix_strides, v_prefix, v_prefix_strides, out, B, K, n_q_heads, n_kv_heads, head_dim,
-                      prefix_keys, dtype);
+                      prefix_keys, dtype, scratch);
   if (!rc)
     rc = check_rows("asrq_prefix_attention", q, q_strides, k_suffix, k_suffix_strides, v_suffix, v_suffix_strides, out, B, K, n_q_heads, n_kv_heads, head_dim,
-                    suffix_keys, dtype);
+                    suffix_keys, dtype, scratch);
   if (rc) return rc;
   if (!suffix_lengths) return fail(ASRQ_ERR_NULL, "asrq_prefix_attention: suffix_lengths must not be NULL");
   if (n_suffix_lengths != 1 && n_suffix_lengths != B * K)
@@ -813,8 +829,16 @@ int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k
   if (B == 0 || K == 0) return ASRQ_OK;
   return rows_attention(q, q_strides, k_prefix, k_prefix_strides, v_prefix, v_prefix_strides, reinterpret_cast<const long long*>(prefix_lengths),
                         suffix_keys > 0 ? k_suffix : nullptr, k_suffix_strides, v_suffix, v_suffix_strides, reinterpret_cast<const long long*>(suffix_lengths),
-                        n_suffix_lengths != 1, out, B, K, n_q_heads, n_kv_heads, head_dim, prefix_keys, suffix_keys, scale, dtype, f->sm_count,
-                        static_cast<cudaStream_t>(stream));
+                        n_suffix_lengths != 1, out, B, K, n_q_heads, n_kv_heads, head_dim, prefix_keys, suffix_keys, scale, dtype,
+                        workspace_bytes >= kStatusBytes ? workspace : nullptr, scratch, scratch_bytes, f->sm_count, static_cast<cudaStream_t>(stream));
+}
+
+size_t asrq_rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t shared_keys, int64_t own_keys) {
+  const DeviceFacts* f;
+  if (B <= 0 || R <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || shared_keys < 0 || own_keys < 0 ||
+      device_facts(&f))
+    return 0;
+  return rows_attention_scratch_bytes(B, R, n_q_heads, n_kv_heads, head_dim, shared_keys, own_keys, f->sm_count);
 }
 
 int asrq_dense_head(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {

@@ -426,6 +426,11 @@ bool scale_of(PyObject* o, int64_t hd, float* scale) {
   *scale = float(PyFloat_AS_DOUBLE(o));
   return true;
 }
+// Memory of an attention call's own (asrq_rows_attention_scratch_bytes)
+at::Tensor rows_scratch(const at::Tensor& q, int64_t key_heads, int64_t shared, int64_t own) {
+  const size_t n = asrq_rows_attention_scratch_bytes(q.size(0), q.size(1), int(q.size(2)), int(key_heads), int(q.size(3)), shared, own);
+  return n ? at::detail::empty_cuda({int64_t(n)}, at::kByte, q.device(), std::nullopt) : at::Tensor();
+}
 inline const int64_t* ints(const at::Tensor* t) { return t ? static_cast<const int64_t*>(t->data_ptr()) : nullptr; }
 
 // cross_attention(q, k, v, lengths or None, scale or None) -> out, or None
@@ -441,14 +446,21 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       !strides_of(*q, 0, 1, 2, qs) || !strides_of(*k, 0, 2, 1, ks) || !strides_of(*v, 0, 2, 1, vs))
     Py_RETURN_NONE;
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(q->device().index()).stream();
+  Held ws;
+  if (!workspace(q->device().index(), stream, 256, &ws)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;  // the Python path makes it
+  }
   at::Tensor out;
   int rc;
   {
     Unlocked unlocked;
     out = fresh(q->sizes(), q->scalar_type(), q->device());
+    const at::Tensor scratch = rows_scratch(*q, k->size(2), k->size(1), 0);
     g_calls.fetch_add(1, std::memory_order_relaxed);
     rc = asrq_cross_attention(q->data_ptr(), qs, k->data_ptr(), ks, v->data_ptr(), vs, ints(len), out.data_ptr(), q->size(0), q->size(1), int(q->size(2)),
-                              int(k->size(2)), int(q->size(3)), k->size(1), scale, dtype, stream);
+                              int(k->size(2)), int(q->size(3)), k->size(1), scale, dtype, ws->data_ptr(), size_t(ws->numel()), scratch.defined() ? scratch.data_ptr() : nullptr,
+                              scratch.defined() ? size_t(scratch.numel()) : 0, stream);
   }
   if (rc) return failed("asrq_cross_attention", rc);
   return THPVariable_Wrap(std::move(out));
@@ -471,14 +483,22 @@ PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       !lengths_of(a[6], q->device(), B, false, &len) || !scale_of(a[7], hd, &scale) || !strides_of(*q, 0, 1, 2, qs))
     Py_RETURN_NONE;
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(q->device().index()).stream();
+  Held ws;
+  if (!workspace(q->device().index(), stream, 256, &ws)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;  // the Python path makes it
+  }
   at::Tensor out;
   int rc;
   {
     Unlocked unlocked;
     out = fresh(q->sizes(), q->scalar_type(), q->device());
+    const at::Tensor scratch = rows_scratch(*q, hkv, kv[0]->size(2), kv[2]->size(2));
     g_calls.fetch_add(1, std::memory_order_relaxed);
     rc = asrq_prefix_attention(q->data_ptr(), qs, kv[0]->data_ptr(), s[0], kv[1]->data_ptr(), s[1], ints(len), kv[2]->data_ptr(), s[2], kv[3]->data_ptr(), s[3],
-                               ints(own), own->numel(), out.data_ptr(), B, K, int(q->size(2)), int(hkv), int(hd), kv[0]->size(2), kv[2]->size(2), scale, dtype, stream);
+                               ints(own), own->numel(), out.data_ptr(), B, K, int(q->size(2)), int(hkv), int(hd), kv[0]->size(2), kv[2]->size(2), scale, dtype,
+                               ws->data_ptr(), size_t(ws->numel()), scratch.defined() ? scratch.data_ptr() : nullptr, scratch.defined() ? size_t(scratch.numel()) : 0,
+                               stream);
   }
   if (rc) return failed("asrq_prefix_attention", rc);
   return THPVariable_Wrap(std::move(out));

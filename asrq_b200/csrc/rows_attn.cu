@@ -16,9 +16,10 @@
 //   values   the lane holds keys 2c, 2c+1, 2c+8, 2c+9 of column g: it loads 8 consecutive dimensions (8g ..) of each of the four keys, pairs the keys by a
 //            byte permutation, and column g of tile j stands for dimension 8g + j.
 // The next chunk's keys are loaded as soon as the scores are done, its values after the product.
+#include <algorithm>
 #include <type_traits>
 
-#include "tcgen05.cuh"
+#include "rows_attn.cuh"
 
 namespace asrq {
 
@@ -27,18 +28,6 @@ int ensure_dynamic_smem(const void* kernel, size_t bytes);
 namespace {
 
 constexpr int kRowsWarps = 8;
-
-struct RowsParams {
-  const uint16_t* q;             // row r of utterance b, head h: q + b * q_b + r * q_r + h * q_h
-  uint16_t* out;                 // B x R x (Hkv * G) x HD
-  const uint16_t *k, *v;         // shared: key t of utterance b, head h at k + b * k_b + h * k_h + t * k_t
-  const uint16_t *k2, *v2;       // own: of row b * R + r
-  const long long *len, *len2;   // B, or NULL for `keys`; one, or B * R
-  long long q_b, q_r, q_h, k_b, k_h, k_t, v_b, v_h, v_t, k2_b, k2_h, k2_t, v2_b, v2_h, v2_t;
-  long long keys, keys2;         // room
-  int len2_many, R, G, Hkv, tiles;
-  float scale_log2;
-};
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -316,6 +305,17 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
     const int r = i / HD, e = i % HD;
     float mx = -INFINITY, acc = 0.f, sum = 0.f;
     for (int w = 0; w < nw; ++w) mx = fmaxf(mx, part[(w * ROWS + r) * PITCH + HD]);
+    const int n_parts = rank == 0 ? p.n_parts : 0, rr = row0 + r;  // what the tensor-core kernel left
+    const float* from = p.parts + (size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + rr / kTcRows) * p.n_parts * part_floats(HD);
+    const int row_at = (rr % kTcRows) * HD + e, ml_at = kTcRows * HD + (rr % kTcRows) * 2;
+    for (int x = 0; x < n_parts; ++x) mx = fmaxf(mx, from[size_t(x) * part_floats(HD) + ml_at]);
+#pragma unroll 4
+    for (int x = 0; x < n_parts; ++x) {
+      const float* d = from + size_t(x) * part_floats(HD);
+      const float wt = d[ml_at + 1] == 0.f ? 0.f : ex2(d[ml_at] - mx);
+      acc = fmaf(wt, d[row_at], acc);
+      sum = fmaf(wt, d[ml_at + 1], sum);
+    }
     for (int w = 0; w < nw; ++w) {
       const float* d = part + (w * ROWS + r) * PITCH;
       const float wt = d[HD + 1] == 0.f ? 0.f : ex2(d[HD] - mx);  // a sum of NaN stays one
@@ -382,10 +382,34 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
 
 }  // namespace
 
+// Whether the tensor-core kernel takes a call, and the parts it divides the keys into (0: it does not).
+// @RULE
+int tc_parts(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, bool own, int sm_count) {
+  const int64_t rows = R * G, tiles = (rows + kTcRows - 1) / kTcRows, items = B * n_kv_heads * tiles, key_tiles = (keys + 63) / 64;
+  if (rows <= (hd == 64 ? 32 : 16) || keys < 64) return 0;
+  const int64_t slots = 2 * sm_count;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 64 && (s == 1 || key_tiles / s >= 4); ++s) {
+    const int64_t cost = (items * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 4) + (s > 1 || own ? 4 + items * s * tiles / slots : 0);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+size_t rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
+  const int G = n_q_heads / n_kv_heads, n = tc_parts(B, R, G, n_kv_heads, hd, keys, keys2 > 0, sm_count);
+  if (n == 0 || (n == 1 && keys2 == 0)) return 0;
+  return size_t(B) * n_kv_heads * ((R * G + kTcRows - 1) / kTcRows) * n * part_floats(hd) * sizeof(float);
+}
+
 int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
                    const void* k2, const int64_t* k2s, const void* v2, const int64_t* v2s, const long long* lengths2, bool lengths2_many, void* out,
-                   int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, float scale, int dtype, int sm_count,
-                   cudaStream_t stream) {
+                   int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, float scale, int dtype, void* status, void* scratch,
+                   size_t scratch_bytes, int sm_count, cudaStream_t stream) {
   RowsParams p = {};
   auto in = [](const void* x) { return static_cast<const uint16_t*>(x); };
   p.q = in(q), p.q_b = qs[0], p.q_r = qs[1], p.q_h = qs[2];
@@ -404,6 +428,20 @@ int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_
   p.R = int(R), p.G = n_q_heads / n_kv_heads, p.Hkv = n_kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   const bool bf16 = dtype == ASRQ_BF16;
+  int parts = status && ((ks[2] && vs[2]) || keys == 1) ? tc_parts(B, R, p.G, n_kv_heads, hd, keys, k2 != nullptr, sm_count) : 0;
+  if (parts > 0) {
+    const size_t part_bytes = size_t(B) * n_kv_heads * ((R * p.G + kTcRows - 1) / kTcRows) * part_floats(hd) * sizeof(float);
+    const bool kept = scratch && scratch_bytes >= part_bytes * parts;
+    if (!kept && !k2) parts = 1;
+    if (kept || !k2) {
+      const bool direct = parts == 1 && !k2;
+      const int rc = rows_attention_tc(p, hd, bf16, B, parts, direct ? nullptr : static_cast<float*>(scratch), status, sm_count, stream);
+      if (rc || direct) return rc;
+      p.parts = static_cast<const float*>(scratch);
+      p.n_parts = parts;
+      p.keys = 0;
+    }
+  }
   if (hd == 128) return bf16 ? launch_rows<128, 1, true>(p, B, sm_count, stream) : launch_rows<128, 1, false>(p, B, sm_count, stream);
   if (R * p.G > 16) return bf16 ? launch_rows<64, 2, true>(p, B, sm_count, stream) : launch_rows<64, 2, false>(p, B, sm_count, stream);
   return bf16 ? launch_rows<64, 1, true>(p, B, sm_count, stream) : launch_rows<64, 1, false>(p, B, sm_count, stream);

@@ -1,0 +1,29 @@
+// What the two kernels of attention over shared keys (rows_attn.cu, rows_attn_tc.cu) have in common.
+#pragma once
+
+#include "tcgen05.cuh"
+
+namespace asrq {
+
+struct RowsParams {
+  const uint16_t* q;             // row r of utterance b, head h: q + b * q_b + r * q_r + h * q_h
+  uint16_t* out;                 // B x R x (Hkv * G) x HD
+  const uint16_t *k, *v;         // shared: key t of utterance b, head h at k + b * k_b + h * k_h + t * k_t
+  const uint16_t *k2, *v2;       // own: of row b * R + r
+  const long long *len, *len2;   // B, or NULL for `keys`; one, or B * R
+  long long q_b, q_r, q_h, k_b, k_h, k_t, v_b, v_h, v_t, k2_b, k2_h, k2_t, v2_b, v2_h, v2_t;
+  long long keys, keys2;         // room
+  int len2_many, R, G, Hkv, tiles;
+  float scale_log2;              // scale * log2 e
+  // What the tensor-core kernel leaves of the shared keys, for a row kernel to join: for every utterance, key head, tile of 128 rows and part
+  // 128 x HD values, then 128 pairs of maximum (as an exponent of two) and sum.
+  const float* parts;
+  int n_parts;
+};
+constexpr int kTcRows = 128;
+__host__ __device__ constexpr int part_floats(int hd) { return kTcRows * (hd + 2); }
+
+// The shared keys of p by tcgen05: the result where there is one part and no own keys, else parts (p.parts ignored).
+int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, int n_parts, float* parts, void* status, int sm_count, cudaStream_t stream);
+
+}  // namespace asrq

@@ -338,11 +338,17 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
  *   q, q_strides   values between utterances, rows and heads;  k, v and theirs: between utterances, heads and positions; multiples of 8;
  *   lengths        B, cut to 0..keys, or NULL for `keys` everywhere; nothing past an utterance's length is read; a row without keys is zero;
  *   out            B x R x n_q_heads x head_dim, contiguous.
- * head_dim 64 or 128; q, k and v 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation.
+ * head_dim 64 or 128; q, k and v 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation; the weights are
+ * rounded to `dtype`.
+ * Many rows run on the tensor-core kernel, whose waits are bounded: it reports in the workspace's status block (256 bytes, the start of any workspace;
+ * asrq_check_status) and, where it divides the keys or the rows have keys of their own, leaves parts in scratch of the call's own
+ * (asrq_rows_attention_scratch_bytes says how much, 0 for none; 16-byte aligned, its contents do not matter; as for
+ * asrq_linearq_a16_scratch it belongs to this call alone until its work is done).  Without a workspace, or without the scratch, other kernels run.
  */
 int asrq_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
                          const int64_t* lengths, void* out, int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t keys, float scale,
-                         int dtype, void* stream);
+                         int dtype, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream);
+size_t asrq_rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t shared_keys, int64_t own_keys);
 
 /*
  * Attention of one decoding step of K beams (or samples) of every utterance that share a prompt: over the prompt's keys, held once
@@ -354,7 +360,7 @@ int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k
                           const int64_t* v_prefix_strides, const int64_t* prefix_lengths, const void* k_suffix, const int64_t* k_suffix_strides,
                           const void* v_suffix, const int64_t* v_suffix_strides, const int64_t* suffix_lengths, int64_t n_suffix_lengths, void* out, int64_t B,
                           int64_t K, int n_q_heads, int n_kv_heads, int head_dim, int64_t prefix_keys, int64_t suffix_keys, float scale, int dtype,
-                          void* stream);
+                          void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream);
 
 /*
  * The floating-point output head of a decoding step: y[M, N] = x[M, K] . w[N, K]^T, all of the 16-bit type `dtype`,

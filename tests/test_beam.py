@@ -48,15 +48,15 @@ def test_reorder_refusals(kw, code):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(q=None), -1), (dict(k=None), -1), (dict(out=None), -1), (dict(dtype=2), -5), (dict(hd=96), -2), (dict(nq=3), -2), (dict(nkv=0), -2), (dict(keys=-1), -2),
-    (dict(B=-1), -2), (dict(R=-1), -2), (dict(qs=I3(8, 8, 4)), -3), (dict(ks=I3(8, -8, 8)), -3), (dict(odd=2), -3),
+    (dict(B=-1), -2), (dict(R=-1), -2), (dict(qs=I3(8, 8, 4)), -3), (dict(ks=I3(8, -8, 8)), -3), (dict(odd=2), -3), (dict(scratch=24), -3),
 ])
 def test_cross_refusals(kw, code):
     keep, p = _ptr()
     s = I3(64, 64, 64)
-    a = dict(q=p, k=p, v=p, out=p, qs=s, ks=s, B=1, R=1, nq=2, nkv=2, hd=64, keys=4, dtype=0, odd=0)
+    a = dict(q=p, k=p, v=p, out=p, qs=s, ks=s, B=1, R=1, nq=2, nkv=2, hd=64, keys=4, dtype=0, odd=0, scratch=None)
     a.update(kw)
     rc = _lib.load().asrq_cross_attention(a["q"] and a["q"] + a["odd"], a["qs"], a["k"], a["ks"], a["v"], s, None, a["out"], a["B"], a["R"], a["nq"], a["nkv"], a["hd"],
-                                          a["keys"], 1.0, a["dtype"], None)
+                                          a["keys"], 1.0, a["dtype"], None, 0, a["scratch"], 0, None)
     assert rc == code and "asrq_cross_attention" in _lib.last_error()
 
 
@@ -66,7 +66,7 @@ def test_prefix_refusals(kw, code):
     s = I3(64, 64, 64)
     a = dict(lengths=p, n=1, ks=p, hd=64, suffix=4)
     a.update(kw)
-    rc = _lib.load().asrq_prefix_attention(p, s, p, s, p, s, None, a["ks"], s, p, s, a["lengths"], a["n"], p, 1, 2, 2, 2, a["hd"], 4, a["suffix"], 1.0, 0, None)
+    rc = _lib.load().asrq_prefix_attention(p, s, p, s, p, s, None, a["ks"], s, p, s, a["lengths"], a["n"], p, 1, 2, 2, 2, a["hd"], 4, a["suffix"], 1.0, 0, None, 0, None, 0, None)
     assert rc == code and "asrq_prefix_attention" in _lib.last_error()
 
 
