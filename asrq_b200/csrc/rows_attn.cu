@@ -9,14 +9,14 @@
 // Bound: the bytes of the keys and values, read once for up to 16 rows (32 with heads of 64) of a key head.  A warp takes a chunk of
 // 32 keys (16 with heads of 128) at a time, all dimensions, and keeps the rows' results in registers; the chunks of an item (utterance, key
 // head, 16 rows) are dealt to the warps of a block or of a cluster of blocks, which meet at the end as (maximum, sum, values).
-// Keys and values go from memory into the operands of mma.sync without passing shared memory, because a contraction may take its index
-// in any order as long as both operands do, and so may the columns of the result:
-//   scores   lane (g, c) of the operand holds dimensions 2c, 2c+1, 2c+8, 2c+9 of key g; it loads 16 consecutive bytes (dimensions 8c .. 8c+7 of 32) and
-//            calls them the four pairs of two steps, for the queries alike;
-//   values   the lane holds keys 2c, 2c+1, 2c+8, 2c+9 of column g: it loads 8 consecutive dimensions (8g ..) of each of the four keys, pairs the keys by a
-//            byte permutation, and column g of tile j stands for dimension 8g + j.
-// The next chunk's keys are loaded as soon as the scores are done, its values after the product.
+// Each warp has three chunks of 8 KB in shared memory and copies for itself, two ahead (in registers, one ahead, a batch of 32 utterances ran at
+// 3.7 TB/s): no block-wide wait until the end.  A contraction may take its index in any order as long as both operands do, and so may the
+// columns of the result, so that lanes read 16 bytes of a key at a time: lane (g, c) of the operand holds dimensions 2c, 2c+1, 2c+8, 2c+9 of
+// key g; it reads 16 consecutive bytes (dimensions 8c .. 8c+7 of 32) and calls them the four pairs of two steps, for the queries alike.  Values
+// are turned on their way by ldmatrix.  The 16-byte pieces of a key lie exchanged so that the eight lanes of a read meet all banks: by 4 in
+// odd keys, those of values by the key.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "rows_attn.cuh"
@@ -28,6 +28,8 @@ int ensure_dynamic_smem(const void* kernel, size_t bytes);
 namespace {
 
 constexpr int kRowsWarps = 8;
+constexpr int kMaxSplit = 16;  // blocks of a cluster
+constexpr int kMaxParts = 64;  // of the tensor-core kernel
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -59,32 +61,58 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// behind the stream dependency, in program order; not kept in L1: a block reads it once
-__device__ __forceinline__ uint4 ld_kv(const uint16_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ void copy16(uint32_t to, const uint16_t* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy16_or_zero(uint32_t to, const uint16_t* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+// four 8 x 8 matrices of 16-bit values, rows at the lanes' addresses, each turned over
+__device__ __forceinline__ void ldmatrix_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// acc + v * 0 of a pair: stays zero but for infinities and NaN
+template <bool BF16>
+__device__ __forceinline__ uint32_t times_zero(uint32_t v, uint32_t acc) {
+  uint32_t r;
+  if constexpr (BF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(acc));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(acc));
+  return r;
+}
+constexpr int kStages = 2, kChunkBytes = 8192;  // a warp's: keys, then values
 
 template <int HD, int MT, bool BF16>
-__global__ void __launch_bounds__(32 * kRowsWarps)
+__global__ void __launch_bounds__(32 * kRowsWarps) __maxnreg__(MT == 1 ? 168 : 240)
 rows_attn_kernel(const __grid_constant__ RowsParams p) {
   constexpr int ROWS = 16 * MT;
   constexpr int KC = HD == 64 ? 32 : 16;              // keys of a chunk
   constexpr int NT = KC / 8, KS = HD / 16, DT = HD / 8;  // score tiles, steps of the scores, tiles of the result
   constexpr int PITCH = HD + 4;
   extern __shared__ __align__(16) float smem[];
-  float* part = smem;                                  // warps x ROWS x PITCH: values, maximum, sum
-  float* mine = smem + kRowsWarps * ROWS * PITCH;      // ROWS x PITCH: the block's
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, nw = blockDim.x >> 5;
+  constexpr int kPart = kStages * kChunkBytes / 4;  // floats from a warp's part to the next: they lie over the chunks
+  static_assert(ROWS * PITCH <= kPart, "a part fits");
+  float* part = smem;                        // of each warp ROWS x PITCH: values, maximum, sum; the sums become weights
+  float* gathered = part + nw * kPart;       // ROWS x HD: this block's share of the result, from every block of the cluster
+  float* stats = gathered + ROWS * HD;       // blocks x ROWS x 2: their maxima and sums
+  float* total_of = stats + 2 * kMaxSplit * ROWS;  // ROWS x 2: the block's (then the cluster's) maximum and sum
+  float* part_w = total_of + 2 * ROWS;       // ROWS x kMaxParts: sums, then weights
+  float* part_m = part_w + ROWS * kMaxParts;
   uint32_t rank, nsplit;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nsplit));
+  // a block's shared memory may be written by another only once it is known to run: arrived here, waited for before the first write
+  if (nsplit > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int item = int(blockIdx.x / nsplit);
   const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.Hkv, b = bh / p.Hkv;
   const int row0 = tile * ROWS, rows = min(ROWS, p.R * p.G - row0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // Behind the tensor-core kernel of the same call only its parts are waited for: it has itself waited for all before it.
+  if (!p.parts) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  }
 
   // the row tile's chunks: the shared keys', then those of each of its rows' own keys, lane i holding the i-th's
   const long long n1 = p.len ? min(max(*(const volatile long long*)(p.len + b), 0ll), p.keys) : p.keys;
@@ -129,104 +157,132 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
     for (int j = 0; j < DT; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
   }
 
-  struct Chunk {
-    const uint16_t *k, *v;  // its first key
+  const uint32_t mem = tc::smem_u32(smem) + uint32_t(warp * kStages * kChunkBytes);
+  constexpr int PER = HD / 8, EACH = 32 / PER;  // pieces of a key; keys the warp's lanes copy at a time
+  const int copy_t = lane / PER, copy_piece = lane % PER;
+  const uint16_t *k1 = p.k + b * p.k_b + h * p.k_h + copy_t * p.k_t + copy_piece * 8, *v1 = p.v + b * p.v_b + h * p.v_h + copy_t * p.v_t + copy_piece * 8;
+  auto copy = [&](int i, int stage) {  // chunk i
+    const uint16_t *k, *v;
     long long kt, vt;
-    int n, seg;             // keys there; -1: shared, else whose
-  };
-  auto chunk_at = [&](int i) {
-    Chunk x;
+    int n;
     if (i < chunks1) {
       const long long t0 = (long long)i * KC;
-      x.k = p.k + b * p.k_b + h * p.k_h + t0 * p.k_t;
-      x.v = p.v + b * p.v_b + h * p.v_h + t0 * p.v_t;
-      x.kt = p.k_t, x.vt = p.v_t;
-      x.n = int(min(n1 - t0, (long long)KC));
-      x.seg = -1;
+      k = k1 + t0 * p.k_t;
+      v = v1 + t0 * p.v_t;
+      kt = p.k_t * EACH, vt = p.v_t * EACH;
+      n = int(min(n1 - t0, (long long)KC));
     } else {
       const int s = __popc(__ballot_sync(0xffffffffu, upto <= i - chunks1));
       const long long t0 = (long long)(i - chunks1 - __shfl_sync(0xffffffffu, upto - chunks2, s)) * KC;
-      const long long n = __shfl_sync(0xffffffffu, len2, s), r = (long long)b * p.R + first + s;
-      x.k = p.k2 + r * p.k2_b + h * p.k2_h + t0 * p.k2_t;
-      x.v = p.v2 + r * p.v2_b + h * p.v2_h + t0 * p.v2_t;
-      x.kt = p.k2_t, x.vt = p.v2_t;
-      x.n = int(min(n - t0, (long long)KC));
-      x.seg = s;
+      const long long len = __shfl_sync(0xffffffffu, len2, s), r = (long long)b * p.R + first + s;
+      k = p.k2 + r * p.k2_b + h * p.k2_h + (t0 + copy_t) * p.k2_t + copy_piece * 8;
+      v = p.v2 + r * p.v2_b + h * p.v2_h + (t0 + copy_t) * p.v2_t + copy_piece * 8;
+      kt = p.k2_t * EACH, vt = p.v2_t * EACH;
+      n = int(min(len - t0, (long long)KC));
     }
-    return x;
-  };
-  uint4 kr[NT][HD / 32], vr[KC / 16][4][HD / 64];
-  auto load_k = [&](const Chunk& x) {
+    const uint32_t at = mem + uint32_t(stage * kChunkBytes);
+    // key u * EACH + copy_t: pieces of keys exchanged by 4 in odd ones, of values by the key's last three bits
+    const uint32_t k_at = at + uint32_t(copy_t * HD * 2 + ((copy_piece ^ ((copy_t & 1) << 2)) * 16));
+    const uint32_t v_at = at + uint32_t(KC * HD * 2 + copy_t * HD * 2), v_piece = uint32_t(copy_piece ^ copy_t) * 16;
+    if (n == KC) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int t = j * 8 + g;
-#pragma unroll
-      for (int ch = 0; ch < HD / 32; ++ch) kr[j][ch] = t < x.n ? ld_kv(x.k + t * x.kt + ch * 32 + c * 8) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  auto load_v = [&](const Chunk& x) {
-#pragma unroll
-    for (int s = 0; s < KC / 16; ++s)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const int t = s * 16 + (a >> 1) * 8 + 2 * c + (a & 1);
-#pragma unroll
-        for (int hh = 0; hh < HD / 64; ++hh) vr[s][a][hh] = t < x.n ? ld_kv(x.v + t * x.vt + hh * 64 + g * 8) : make_uint4(0, 0, 0, 0);
+      for (int u = 0; u < KC / EACH; ++u, k += kt, v += vt) {
+        copy16(k_at + u * EACH * HD * 2, k);
+        copy16(v_at + u * EACH * HD * 2 + (v_piece ^ (((u * EACH) & 7) * 16)), v);
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < KC / EACH; ++u, k += kt, v += vt) {
+        const bool there = u * EACH + copy_t < n;
+        copy16_or_zero(k_at + u * EACH * HD * 2, there ? k : p.q, there);
+        copy16_or_zero(v_at + u * EACH * HD * 2 + (v_piece ^ (((u * EACH) & 7) * 16)), there ? v : p.q, there);
+      }
+    }
   };
   const int step = int(nsplit) * nw;
   int at = int(rank) * nw + warp;
-  Chunk cur, next;
-  if (at < total) {
-    cur = chunk_at(at);
-    load_k(cur);
-    load_v(cur);
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (at + s * step < total) copy(at + s * step, s);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
+  int stage = 0;
 #pragma unroll 1
   for (; at < total; at += step) {
-    const bool more = at + step < total;
-    if (more) next = chunk_at(at + step);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncwarp();  // the other lanes' copies too; and the stage that is filled next has been read
+    if (at + (kStages - 1) * step < total) copy(at + (kStages - 1) * step, stage == 0 ? kStages - 1 : stage - 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    int n, seg = -1;  // keys there; whose: -1 all rows'
+    if (at < chunks1) {
+      n = int(min(n1 - (long long)at * KC, (long long)KC));
+    } else {
+      seg = __popc(__ballot_sync(0xffffffffu, upto <= at - chunks1));
+      n = int(min(__shfl_sync(0xffffffffu, len2, seg) - (long long)(at - chunks1 - __shfl_sync(0xffffffffu, upto - chunks2, seg)) * KC, (long long)KC));
+    }
+    const uint32_t keys_at = mem + uint32_t(stage * kChunkBytes), values_at = keys_at + KC * HD * 2;
     float s[MT][NT][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int j = 0; j < NT; ++j) {
+      float odd[MT][4] = {};  // two chains of products
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
+      for (int mt = 0; mt < MT; ++mt) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
 #pragma unroll
-        for (int ch = 0; ch < HD / 32; ++ch) {
-          mma16816<BF16>(s[mt][j], qf[mt][2 * ch], kr[j][ch].x, kr[j][ch].y);
-          mma16816<BF16>(s[mt][j], qf[mt][2 * ch + 1], kr[j][ch].z, kr[j][ch].w);
+      for (int ch = 0; ch < HD / 32; ++ch) {
+        const uint4 k = tc::ld_shared_v4(keys_at + uint32_t((j * 8 + g) * HD * 2 + (((ch * 4 + c) ^ ((g & 1) << 2)) * 16)));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          mma16816<BF16>(s[mt][j], qf[mt][2 * ch], k.x, k.y);
+          mma16816<BF16>(odd[mt], qf[mt][2 * ch + 1], k.z, k.w);
         }
       }
-    if (more) load_k(next);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][j][e] += odd[mt][e];
+    }
     uint32_t pr[MT][NT][2];
+    const bool some = n < KC || seg >= 0;  // scores that do not count
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
+      if (some) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j * 8 + 2 * c + (e & 1) >= n || (seg >= 0 && seg != own[mt][e >> 1])) s[mt][j][e] = -INFINITY;
+            else s[mt][j][e] *= p.scale_log2;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][j][e] *= p.scale_log2;
+      }
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool live = j * 8 + 2 * c + (e & 1) < cur.n && (cur.seg < 0 || cur.seg == own[mt][e >> 1]);
-          s[mt][j][e] = live ? s[mt][j][e] * p.scale_log2 : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], s[mt][j][e]);
-        }
-      float base[2];
+        for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[mt][j][e]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
         mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
-        const float now = fmaxf(m[mt][half], mx[half]);
-        base[half] = now == -INFINITY ? 0.f : now;  // no key of this row yet
-        const float corr = ex2(m[mt][half] - base[half]);
-        m[mt][half] = now;
-        l[mt][half] *= corr;
+      }
+      // The reference exponent of a row moves only when its maximum has grown by more than 8 (a weight stays below 2^8).
+      if (__any_sync(0xffffffffu, mx[0] > m[mt][0] + 8.f || mx[1] > m[mt][1] + 8.f)) {
 #pragma unroll
-        for (int j = 0; j < DT; ++j) {
-          o[mt][j][2 * half] *= corr;
-          o[mt][j][2 * half + 1] *= corr;
+        for (int half = 0; half < 2; ++half) {
+          const float now = fmaxf(m[mt][half], mx[half]), corr = now == m[mt][half] ? 1.f : ex2(m[mt][half] - now);
+          m[mt][half] = now;
+          l[mt][half] *= corr;
+#pragma unroll
+          for (int j = 0; j < DT; ++j) {
+            o[mt][j][2 * half] *= corr;
+            o[mt][j][2 * half + 1] *= corr;
+          }
         }
       }
+      const float base[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0], m[mt][1] == -INFINITY ? 0.f : m[mt][1]};  // (no key of this row yet)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -237,40 +293,53 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
           l[mt][half] += r.x + r.y;
         }
     }
-    // Own keys are those of some rows only: the others' weights are zero, but a zero times an infinity is not, so their results stay out.
-    auto product = [&](auto shared) {
+    // the values of 16 keys and 16 dimensions at a time, turned: two operands of two registers
+    uint32_t vr[KC / 16][DT / 2][4];
+    bool finite = true;
 #pragma unroll
-      for (int hh = 0; hh < HD / 64; ++hh)
+    for (int st = 0; st < KC / 16; ++st)
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+      for (int j = 0; j < DT / 2; ++j) {
+        const int t = st * 16 + (lane & 15), piece = 2 * j + (lane >> 4);
+        ldmatrix_turned(vr[st][j], values_at + uint32_t(t * HD * 2 + ((piece ^ (t & 7)) * 16)));
+      }
+    // Own keys are those of some rows only: the others' weights are zero, but a zero times an infinity is not, so then their results stay out.
+    if (seg >= 0) {
+      uint32_t zero = 0;
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
-            const int j = hh * 8 + 2 * w + odd;
-            float add[MT][4] = {};
+      for (int st = 0; st < KC / 16; ++st)
 #pragma unroll
-            for (int st = 0; st < KC / 16; ++st) {
-              auto word = [&](int a) { return w == 0 ? vr[st][a][hh].x : w == 1 ? vr[st][a][hh].y : w == 2 ? vr[st][a][hh].z : vr[st][a][hh].w; };
-              const uint32_t b0 = prmt(word(0), word(1), odd ? 0x7632u : 0x5410u), b1 = prmt(word(2), word(3), odd ? 0x7632u : 0x5410u);
+        for (int j = 0; j < DT / 2; ++j)
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                const uint32_t a[4] = {pr[mt][2 * st][0], pr[mt][2 * st][1], pr[mt][2 * st + 1][0], pr[mt][2 * st + 1][1]};
-                mma16816<BF16>(shared.value ? o[mt][j] : add[mt], a, b0, b1);
-              }
-            }
-            if (!shared.value) {
+          for (int x = 0; x < 4; ++x) zero = times_zero<BF16>(vr[st][j][x], zero);
+      finite = __all_sync(0xffffffffu, (zero & 0x7fff7fffu) == 0);
+    }
+    auto product = [&](auto plain) {
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
+      for (int j = 0; j < DT; ++j) {
+        float add[MT][4] = {};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (cur.seg == own[mt][e >> 1]) o[mt][j][e] += add[mt][e];
-            }
+        for (int st = 0; st < KC / 16; ++st)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t a[4] = {pr[mt][2 * st][0], pr[mt][2 * st][1], pr[mt][2 * st + 1][0], pr[mt][2 * st + 1][1]};
+            mma16816<BF16>(plain.value ? o[mt][j] : add[mt], a, vr[st][j / 2][(j & 1) * 2], vr[st][j / 2][(j & 1) * 2 + 1]);
           }
+        if (!plain.value) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (seg == own[mt][e >> 1]) o[mt][j][e] += add[mt][e];
+        }
+      }
     };
-    if (cur.seg < 0) product(std::true_type{});
+    if (finite) product(std::true_type{});
     else product(std::false_type{});
-    if (more) load_v(next);
-    cur = next;
+    stage = stage == kStages - 1 ? 0 : stage + 1;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();  // the chunks' memory is the part's now
   // the warps' parts, the block's, the cluster's
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -280,92 +349,187 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
       l[mt][half] += __shfl_xor_sync(0xffffffffu, l[mt][half], 2);
       const int r = mt * 16 + half * 8 + g;
       if (r >= rows) continue;
-      float* d = part + (warp * ROWS + r) * PITCH;
+      float* d = part + warp * kPart + r * PITCH;
 #pragma unroll
-      for (int hh = 0; hh < HD / 64; ++hh)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)  // columns 2c and 2c + 1 of the tiles: dimensions 16c .. and 16c + 8 ..
-#pragma unroll
-          for (int q4 = 0; q4 < 2; ++q4) {
-            const int j = hh * 8 + q4 * 4, x = 2 * half + e;
-            *reinterpret_cast<float4*>(d + hh * 64 + 16 * c + 8 * e + 4 * q4) = make_float4(o[mt][j][x], o[mt][j + 1][x], o[mt][j + 2][x], o[mt][j + 3][x]);
-          }
+      for (int j = 0; j < DT; ++j) *reinterpret_cast<float2*>(d + j * 8 + 2 * c) = make_float2(o[mt][j][2 * half], o[mt][j][2 * half + 1]);
       if (c == 0) {
         d[HD] = m[mt][half];
         d[HD + 1] = l[mt][half];
       }
     }
+  // What the tensor-core kernel left, every block of the cluster its share of the parts.
+  const int n_parts = p.parts ? (p.n_parts - int(rank) + int(nsplit) - 1) / int(nsplit) : 0;
+  const float* from = nullptr;
+  if (p.parts) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // (a row tile does not cross a tile of 128)
+    from = behind_wait(p.parts + ((size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + row0 / kTcRows) * p.n_parts + rank) * part_floats(HD));
+    for (int i = threadIdx.x; i < rows * n_parts; i += blockDim.x) {
+      const int r = i / n_parts, x = i % n_parts;
+      const float2 ml = *reinterpret_cast<const float2*>(from + size_t(x) * nsplit * part_floats(HD) + kTcRows * HD + (row0 % kTcRows + r) * 2);
+      part_m[r * kMaxParts + x] = ml.x;
+      part_w[r * kMaxParts + x] = ml.y;
+    }
+  }
+  __syncthreads();
+  // a warp a row: its maximum and sum over warps and parts, and their weights (a sum of NaN stays one)
+  for (int r = warp; r < rows; r += nw) {
+    float mw = -INFINITY, lw = 0.f, mx;
+    if (lane < nw) {
+      mw = part[lane * kPart + r * PITCH + HD];
+      lw = part[lane * kPart + r * PITCH + HD + 1];
+    }
+    mx = mw;
+    for (int x = lane; x < n_parts; x += 32) mx = fmaxf(mx, part_m[r * kMaxParts + x]);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ww = lw == 0.f ? 0.f : ex2(mw - mx);
+    float sum = ww * lw;
+    for (int x = lane; x < n_parts; x += 32) {
+      const float l = part_w[r * kMaxParts + x], wt = l == 0.f ? 0.f : ex2(part_m[r * kMaxParts + x] - mx);
+      sum = fmaf(wt, l, sum);
+      part_w[r * kMaxParts + x] = wt;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane < nw) part[lane * kPart + r * PITCH + HD + 1] = ww;
+    if (lane == 0) {
+      total_of[2 * r] = mx;
+      total_of[2 * r + 1] = sum;
+    }
+  }
+  if (nsplit > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   __syncthreads();
   const int Hq = p.Hkv * p.G;
-  auto put = [&](int r, int e, float v, float sum) {  // element e of the tile's row r
+  auto put4 = [&](int r, int e, float4 v, float sum) {  // elements e .. e + 3 of the tile's row r
     const int rr = row0 + r;
-    p.out[((size_t(b) * p.R + rr / p.G) * Hq + h * p.G + rr % p.G) * HD + e] = float_to_out16(sum > 0.f || sum != sum ? v / sum : 0.f, BF16);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.R + rr / p.G) * Hq + h * p.G + rr % p.G) * HD + e) =
+        make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
   };
-  for (int i = threadIdx.x; i < rows * HD; i += blockDim.x) {
-    const int r = i / HD, e = i % HD;
-    float mx = -INFINITY, acc = 0.f, sum = 0.f;
-    for (int w = 0; w < nw; ++w) mx = fmaxf(mx, part[(w * ROWS + r) * PITCH + HD]);
-    const int n_parts = rank == 0 ? p.n_parts : 0, rr = row0 + r;  // what the tensor-core kernel left
-    const float* from = p.parts + (size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + rr / kTcRows) * p.n_parts * part_floats(HD);
-    const int row_at = (rr % kTcRows) * HD + e, ml_at = kTcRows * HD + (rr % kTcRows) * 2;
-    for (int x = 0; x < n_parts; ++x) mx = fmaxf(mx, from[size_t(x) * part_floats(HD) + ml_at]);
+  // Four elements a thread.  In a cluster a block finishes every nsplit-th of them: the others send it theirs.
+  constexpr int Q4 = HD / 4;
+  for (int i = threadIdx.x; i < rows * Q4; i += blockDim.x) {
+    const int r = i / Q4, e = (i % Q4) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, const float4& v) {
+      acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
+    };
 #pragma unroll 4
-    for (int x = 0; x < n_parts; ++x) {
-      const float* d = from + size_t(x) * part_floats(HD);
-      const float wt = d[ml_at + 1] == 0.f ? 0.f : ex2(d[ml_at] - mx);
-      acc = fmaf(wt, d[row_at], acc);
-      sum = fmaf(wt, d[ml_at + 1], sum);
-    }
-    for (int w = 0; w < nw; ++w) {
-      const float* d = part + (w * ROWS + r) * PITCH;
-      const float wt = d[HD + 1] == 0.f ? 0.f : ex2(d[HD] - mx);  // a sum of NaN stays one
-      acc = fmaf(wt, d[e], acc);
-      sum = fmaf(wt, d[HD + 1], sum);
-    }
+    for (int w = 0; w < nw; ++w) add(part[w * kPart + r * PITCH + HD + 1], *reinterpret_cast<const float4*>(part + w * kPart + r * PITCH + e));
+#pragma unroll 8
+    for (int x = 0; x < n_parts; ++x)
+      add(part_w[r * kMaxParts + x], *reinterpret_cast<const float4*>(from + size_t(x) * nsplit * part_floats(HD) + (row0 % kTcRows + r) * HD + e));
     if (nsplit == 1) {
-      put(r, e, acc, sum);
+      put4(r, e, acc, total_of[2 * r + 1]);
     } else {
-      mine[r * PITCH + e] = acc;
-      if (e == 0) {
-        mine[r * PITCH + HD] = mx;
-        mine[r * PITCH + HD + 1] = sum;
-      }
+      const uint32_t to = tc::mapa(tc::smem_u32(gathered + (rank * (ROWS * Q4 / nsplit) + i / nsplit) * 4), uint32_t(i) % nsplit);
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(acc.x), "f"(acc.y), "f"(acc.z), "f"(acc.w) : "memory");
     }
   }
   if (nsplit == 1) return;
-  tc::cluster_sync();  // every block's part is there
-  const uint32_t base = tc::smem_u32(mine);
-  for (int i = int(rank) * int(blockDim.x) + threadIdx.x; i < rows * HD; i += int(nsplit) * int(blockDim.x)) {
-    const int r = i / HD, e = i % HD;
-    float mx = -INFINITY, acc = 0.f, sum = 0.f;
-    for (uint32_t x = 0; x < nsplit; ++x) mx = fmaxf(mx, tc::ld_dsmem_f32(tc::mapa(base + uint32_t(r * PITCH + HD) * 4u, x)));
-    for (uint32_t x = 0; x < nsplit; ++x) {
-      const uint32_t d = tc::mapa(base + uint32_t(r * PITCH) * 4u, x);
-      const float part_sum = tc::ld_dsmem_f32(d + HD * 4u + 4u), wt = part_sum == 0.f ? 0.f : ex2(tc::ld_dsmem_f32(d + HD * 4u) - mx);
-      acc = fmaf(wt, tc::ld_dsmem_f32(d + uint32_t(e) * 4u), acc);
-      sum = fmaf(wt, part_sum, sum);
-    }
-    put(r, e, acc, sum);
+  for (int i = threadIdx.x; i < rows * int(nsplit); i += blockDim.x) {
+    const int r = i / int(nsplit);
+    const uint32_t to = tc::mapa(tc::smem_u32(stats + (rank * ROWS + r) * 2), uint32_t(i) % nsplit);
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(total_of[2 * r]), "f"(total_of[2 * r + 1]) : "memory");
   }
-  tc::cluster_sync();  // none leaves while another reads its part
+  tc::cluster_sync();  // everything has arrived, and nobody reads another's any more
+  for (int i = int(rank) + threadIdx.x * int(nsplit); i < rows * Q4; i += int(blockDim.x) * int(nsplit)) {
+    const int r = i / Q4, e = (i % Q4) * 4;
+    float mx = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (uint32_t x = 0; x < nsplit; ++x) mx = fmaxf(mx, stats[(x * ROWS + r) * 2]);
+#pragma unroll 4
+    for (uint32_t x = 0; x < nsplit; ++x) {
+      const float2 ml = *reinterpret_cast<const float2*>(stats + (x * ROWS + r) * 2);
+      const float4 v = *reinterpret_cast<const float4*>(gathered + (x * (ROWS * Q4 / nsplit) + i / nsplit) * 4);
+      const float w = ml.y == 0.f ? 0.f : ex2(ml.x - mx);
+      sum = fmaf(w, ml.y, sum);
+      acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
+    }
+    put4(r, e, acc, sum);
+  }
+}
+
+template <int HD, int MT>
+size_t rows_smem(int warps, bool parts) {
+  constexpr int ROWS = 16 * MT;
+  return size_t(warps) * kStages * kChunkBytes + (ROWS * HD + 2 * kMaxSplit * ROWS + 2 * ROWS + (parts ? size_t(2) * ROWS * kMaxParts : 0)) * 4;
+}
+
+// Blocks of `warps` warps, in clusters of `split`, that the device holds at once
+template <int HD, int MT, bool BF16>
+int64_t resident_blocks(int split, int warps, bool parts, int sm_count) {
+  static std::atomic<int> known[2][kMaxSplit + 1][kRowsWarps + 1];  // one kind of device: asked once per process
+  std::atomic<int>& k = known[parts][split][warps];
+  int n = k.load(std::memory_order_relaxed);
+  if (n) return n;
+  auto kern = rows_attn_kernel<HD, MT, BF16>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(split));
+  cfg.blockDim = dim3(32 * warps);
+  cfg.dynamicSmemBytes = rows_smem<HD, MT>(warps, parts);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = std::max(1, sm_count / split);
+  }
+  k.store(n * split, std::memory_order_relaxed);
+  return n * split;
+}
+
+struct RowsChoice {
+  int split, warps;
+  int64_t cost;
+};
+// Blocks an item and warps a block: the least (waves of resident blocks) x (chunks a warp walks, and 3 for a block's start and end, one
+// more in a cluster).  us by (warps, blocks): 1x5 rows on 1500 keys (6, 8) 5.5, (8, 4) 5.7, (4, 4) 6.0, (8, 8) 9.2 in two waves; 16x5 on 150..1500
+// (4, 1) 18.1, (6, 1) 17.5, (8, 1) 20.3, (4, 2) 20.6; 64x5 on 258 + 65 (6, 1) 34.4, (2, 1) 38.1, (4, 1) 42.3; 32x5 on 1500 (2, 1) 41.8, (4, 1) 44.9.
+template <int HD, int MT, bool BF16>
+RowsChoice choose_rows(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys, int64_t keys2, bool parts, int sm_count) {
+  constexpr int ROWS = 16 * MT, KC = HD == 64 ? 32 : 16;
+  const int64_t items = B * n_kv_heads * ((R * G + ROWS - 1) / ROWS);
+  const int64_t chunks = (keys + KC - 1) / KC + std::min<int64_t>((ROWS - 1) / G + 1, R) * ((keys2 + KC - 1) / KC);
+  RowsChoice best = {1, kRowsWarps, INT64_MAX};
+  for (int s = 1; s <= kMaxSplit; s *= 2)
+    for (int w = kRowsWarps; w >= 1; --w) {
+      const int64_t slots = resident_blocks<HD, MT, BF16>(s, w, parts, sm_count);
+      const int64_t cost = (items * s + slots - 1) / slots * ((chunks + s * w - 1) / (s * w) + (s > 1 ? 4 : 3));
+      if (cost < best.cost) best = {s, w, cost};
+    }
+  return best;
+}
+
+template <int HD, int MT, bool BF16>
+int allow_rows() {  // what the occupancy query and the launch need set
+  auto kern = rows_attn_kernel<HD, MT, BF16>;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), rows_smem<HD, MT>(kRowsWarps, true));
+  if (rc) return rc;
+  ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  return ASRQ_OK;
 }
 
 template <int HD, int MT, bool BF16>
 int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
-  constexpr int ROWS = 16 * MT, KC = HD == 64 ? 32 : 16;
-  constexpr size_t smem = size_t(kRowsWarps + 1) * ROWS * (HD + 4) * 4;
+  constexpr int ROWS = 16 * MT;
   p.tiles = (p.R * p.G + ROWS - 1) / ROWS;
   const int64_t items = B * p.Hkv * p.tiles;
   auto kern = rows_attn_kernel<HD, MT, BF16>;
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem);
+  const int rc = allow_rows<HD, MT, BF16>();
   if (rc) return rc;
-  // blocks an item: until the chip is full, or a warp has a single chunk
-  const int64_t chunks = (p.keys + KC - 1) / KC + (p.k2 ? (p.keys2 + KC - 1) / KC : 0);
-  int split = 1;
-  while (split < 8 && items * split * 2 <= sm_count * 5 / 4 && chunks > split * kRowsWarps) split *= 2;
+  const RowsChoice choice = choose_rows<HD, MT, BF16>(B, p.R, p.G, p.Hkv, p.keys, p.k2 ? p.keys2 : 0, p.parts != nullptr, sm_count);
+  const int split = choice.split, warps = choice.warps;
+  const size_t smem = rows_smem<HD, MT>(warps, p.parts != nullptr);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(items * split));
-  cfg.blockDim = dim3(32 * kRowsWarps);
+  cfg.blockDim = dim3(32 * warps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -382,28 +546,50 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
 
 }  // namespace
 
-// Whether the tensor-core kernel takes a call, and the parts it divides the keys into (0: it does not).
-// @RULE
-int tc_parts(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, bool own, int sm_count) {
-  const int64_t rows = R * G, tiles = (rows + kTcRows - 1) / kTcRows, items = B * n_kv_heads * tiles, key_tiles = (keys + 63) / 64;
-  if (rows <= (hd == 64 ? 32 : 16) || keys < 64) return 0;
-  const int64_t slots = 2 * sm_count;
-  int best = 1;
-  int64_t least = INT64_MAX;
-  for (int s = 1; s <= 64 && (s == 1 || key_tiles / s >= 4); ++s) {
-    const int64_t cost = (items * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 4) + (s > 1 || own ? 4 + items * s * tiles / slots : 0);
+// The row kernel's time in us, by its units above: 1.2 each, more with many dimensions or rows to a warp (measured: 1.1 to 1.5, 1.2 to 1.5, 1.6 to 1.75).
+double rows_estimate(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, int64_t keys2, bool parts, int sm_count) {
+  if (hd == 128) return 1.3 * double(choose_rows<128, 1, false>(B, R, G, n_kv_heads, keys, keys2, parts, sm_count).cost);
+  if (R * G > 16) return 1.65 * double(choose_rows<64, 2, false>(B, R, G, n_kv_heads, keys, keys2, parts, sm_count).cost);
+  return 1.2 * double(choose_rows<64, 1, false>(B, R, G, n_kv_heads, keys, keys2, parts, sm_count).cost);
+}
+
+// Whether the tensor-core kernel takes a call, and how it divides it.  It walks tiles of keys at 1.3 us a wave of blocks, with 3 for a block's start
+// and end, however few of the 128 rows there are; items that fill the chip are left whole, the rest divided so that it is filled once
+// more, and a join is worth about 4.  us, the row kernel first: heads of 64 on 1500 keys, 16 utterances of 5 rows 23 | 34, 20 rows 45 | 37, 64 rows
+// 76 | 38; 4 utterances of 32 rows 16 | 18, 40 rows 24 | 18; 1 of 64 11 | 14; heads of 128 on 6000 keys, 16 utterances of 20 rows 78 | 73, 64 rows 164 | 79.
+TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
+  const int64_t rows = R * G, tiles = (rows + kTcRows - 1) / kTcRows, items = B * n_kv_heads * tiles, step = hd == 64 ? 96 : 64;
+  const int64_t key_tiles = (keys + step - 1) / step, slots = 2 * sm_count;
+  const bool own = keys2 > 0;
+  if (rows <= 16 || keys < 64) return {0, 0};
+  const int64_t whole = own ? 0 : items / slots * slots, rest = items - whole, first = whole / slots * (key_tiles + 3);
+  TcPlan plan = {own ? 0 : items, own ? 0 : 1};
+  int64_t least = rest == 0 ? 0 : own ? INT64_MAX : key_tiles + 3;
+  for (int s = own ? 1 : 2; s <= kMaxParts && rest > 0 && (s == 1 || key_tiles >= 2 * s); ++s) {
+    const int64_t cost = (rest * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 3) + 4 + s / 8;
     if (cost < least) {
       least = cost;
-      best = s;
+      plan = {whole, s};
     }
   }
-  return best;
+  double us = 1.3 * double(first + least);
+  if (own) us += rows_estimate(B, R, G, n_kv_heads, hd, 0, keys2, true, sm_count);
+  return us < rows_estimate(B, R, G, n_kv_heads, hd, keys, keys2, false, sm_count) ? plan : TcPlan{0, 0};
+}
+int allow_all() {
+  int rc = allow_rows<64, 1, false>();
+  if (!rc) rc = allow_rows<64, 2, false>();
+  if (!rc) rc = allow_rows<128, 1, false>();
+  return rc;
+}
+size_t part_bytes(int64_t B, int64_t R, int G, int n_kv_heads, int hd, const TcPlan& plan) {
+  const int64_t items = B * n_kv_heads * ((R * G + kTcRows - 1) / kTcRows);
+  return size_t(items - plan.whole) * plan.split * part_floats(hd) * sizeof(float);
 }
 
 size_t rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
-  const int G = n_q_heads / n_kv_heads, n = tc_parts(B, R, G, n_kv_heads, hd, keys, keys2 > 0, sm_count);
-  if (n == 0 || (n == 1 && keys2 == 0)) return 0;
-  return size_t(B) * n_kv_heads * ((R * G + kTcRows - 1) / kTcRows) * n * part_floats(hd) * sizeof(float);
+  const int G = n_q_heads / n_kv_heads;
+  return allow_all() ? 0 : part_bytes(B, R, G, n_kv_heads, hd, tc_plan(B, R, G, n_kv_heads, hd, keys, keys2, sm_count));
 }
 
 int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
@@ -428,17 +614,19 @@ int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_
   p.R = int(R), p.G = n_q_heads / n_kv_heads, p.Hkv = n_kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   const bool bf16 = dtype == ASRQ_BF16;
-  int parts = status && ((ks[2] && vs[2]) || keys == 1) ? tc_parts(B, R, p.G, n_kv_heads, hd, keys, k2 != nullptr, sm_count) : 0;
-  if (parts > 0) {
-    const size_t part_bytes = size_t(B) * n_kv_heads * ((R * p.G + kTcRows - 1) / kTcRows) * part_floats(hd) * sizeof(float);
-    const bool kept = scratch && scratch_bytes >= part_bytes * parts;
-    if (!kept && !k2) parts = 1;
+  TcPlan plan = {0, 0};
+  int rc = allow_all();
+  if (rc) return rc;
+  if (status && ((ks[2] && vs[2]) || keys == 1)) plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
+  if (plan.split > 0) {
+    const size_t need = part_bytes(B, R, p.G, n_kv_heads, hd, plan);
+    const bool kept = need == 0 || (scratch && scratch_bytes >= need);
+    if (!kept && !k2) plan = {B * n_kv_heads * ((R * p.G + kTcRows - 1) / kTcRows), 1};
     if (kept || !k2) {
-      const bool direct = parts == 1 && !k2;
-      const int rc = rows_attention_tc(p, hd, bf16, B, parts, direct ? nullptr : static_cast<float*>(scratch), status, sm_count, stream);
-      if (rc || direct) return rc;
+      rc = rows_attention_tc(p, hd, bf16, B, plan, need && kept ? static_cast<float*>(scratch) : nullptr, !k2, status, stream);
+      if (rc || !k2) return rc;
       p.parts = static_cast<const float*>(scratch);
-      p.n_parts = parts;
+      p.n_parts = plan.split;
       p.keys = 0;
     }
   }

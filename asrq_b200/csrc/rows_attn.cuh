@@ -23,7 +23,14 @@ struct RowsParams {
 constexpr int kTcRows = 128;
 __host__ __device__ constexpr int part_floats(int hd) { return kTcRows * (hd + 2); }
 
-// The shared keys of p by tcgen05: the result where there is one part and no own keys, else parts (p.parts ignored).
-int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, int n_parts, float* parts, void* status, int sm_count, cudaStream_t stream);
+// How the tensor-core kernel divides a call's items (utterance, key head, 128 rows): the first `whole` have a block each, the keys of the others
+// are divided among `split`, each of which leaves a part.  split 0: the call is not for it.
+struct TcPlan {
+  int64_t whole;
+  int split;
+};
+
+// The shared keys of p by tcgen05.  join: the parts are joined to results; else they are left for a row kernel (whole is 0 then).
+int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, bool join, void* status, cudaStream_t stream);
 
 }  // namespace asrq

@@ -1,11 +1,11 @@
 // Attention of many query rows over keys that they share, on the 5th-generation tensor cores: the tokens of a prompt over an encoder's
 // states, or the rows of many beams or samples over their prompt.
 //
-// A block holds 128 rows (all query heads of a key head, so several tokens or beams) and walks its keys 64 at a time: S = Q K^T into tensor
-// memory, a thread per row reads its 64 scores, and writes the weights 2^(scale' s - m) back over them in 16 bits, from where
-// O += P V takes them as its first operand.  K arrives by TMA as rows of the contraction, V as it lies, dimensions contiguous, which the
-// second operand's descriptor calls MN-major.  Two score buffers: S of the next keys is done while these are exponentiated; two blocks an
-// SM fill each other's waits.
+// A block holds 128 rows (all query heads of a key head, so several tokens or beams) and walks its keys 96 (64 with 128 dimensions) at a
+// time: S = Q K^T into tensor memory, a thread per row reads its scores, and writes the weights 2^(scale' s - m) in 16 bits to tensor memory
+// too, from where O += P V takes them as its first operand.  K arrives by TMA as rows of the contraction, V as it lies, dimensions
+// contiguous, which the second operand's descriptor calls MN-major.  The next S is on its way as soon as the scores are in registers, and
+// two blocks an SM fill each other's waits.
 // The reference exponent m of a row moves only when its maximum has grown by more than 8 (a weight stays below 2^8, a sum in 32 bits has
 // room for that): O is scaled at the first tiles and hardly ever after.
 //
@@ -18,8 +18,6 @@ int ensure_dynamic_smem(const void* kernel, size_t bytes);
 
 namespace {
 
-constexpr int kKeys = 64;  // of a tile
-
 struct FlashParams {
   const uint16_t* q;
   uint16_t* out;
@@ -27,17 +25,18 @@ struct FlashParams {
   float* parts;
   unsigned* status;
   long long q_b, q_r, q_h, keys;
-  int R, G, Hkv, tiles, split, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
+  int R, G, Hkv, tiles, whole, split, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
   float scale_log2;  // not negative
   uint32_t q_flip;   // the sign bits of a query pair where the scale is
 };
 
 template <int HD>
 struct FlashLayout {
-  static constexpr int kStages = HD == 64 ? 4 : 2;
+  static constexpr int kKeys = HD == 64 ? 96 : 64;  // of a tile: tensor memory has 256 columns for S (32 bits), P (16 bits) and O of a block
+  static constexpr int kStages = HD == 64 ? 3 : 2;
   static constexpr int kQ = kTcRows * HD * 2, kTile = kKeys * HD * 2;
   static constexpr int kK = kQ, kV = kQ + kStages * kTile, kBars = kQ + 2 * kStages * kTile;
-  static constexpr int kBytes = kBars + (4 * kStages + 5) * 8 + 16 + 1024;  // 1024: the base is aligned to it
+  static constexpr int kBytes = kBars + (4 * kStages + 4) * 8 + 16 + 1024;  // 1024: the base is aligned to it
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -69,6 +68,18 @@ __device__ __forceinline__ float ex2f(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// registers to tensor memory: 32 lanes of the warp's quadrant x 16 columns
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
@@ -88,8 +99,9 @@ template <int HD, bool BF16>
 __global__ void __launch_bounds__(192, 2)
 flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FlashParams p) {
   using L = FlashLayout<HD>;
-  constexpr int ST = L::kStages, HALVES = HD / 64;
-  constexpr uint32_t kOut = 128;  // tensor memory: two score buffers of 64 columns, then the result
+  constexpr int ST = L::kStages, HALVES = HD / 64, kKeys = L::kKeys;
+  constexpr uint32_t kP = kKeys, kOut = 256 - HD;  // columns of tensor memory: the scores from 0, the weights, the result
+  static_assert(kP + kKeys / 2 <= kOut, "256 columns");
   extern __shared__ uint8_t flash_smem[];
   const uint32_t base = (tc::smem_u32(flash_smem) + 1023u) & ~1023u;
   uint8_t* smem = flash_smem + (base - tc::smem_u32(flash_smem));
@@ -99,21 +111,19 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
   auto k_free = [&](int s) { return bar(ST + s); };
   auto v_full = [&](int s) { return bar(2 * ST + s); };
   auto v_free = [&](int s) { return bar(3 * ST + s); };
-  auto s_full = [&](int i) { return bar(4 * ST + i); };
-  auto p_full = [&](int i) { return bar(4 * ST + 2 + i); };
-  const uint32_t o_done = bar(4 * ST + 4);
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kBars + (4 * ST + 5) * 8);
+  const uint32_t s_full = bar(4 * ST), s_free = bar(4 * ST + 1), p_full = bar(4 * ST + 2), o_done = bar(4 * ST + 3);
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kBars + (4 * ST + 4) * 8);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4 * ST + 2; ++i) tc::mbar_init(bar(i), 1);
-    tc::mbar_init(p_full(0), 4);
-    tc::mbar_init(p_full(1), 4);
-    tc::mbar_init(o_done, 1);
+    for (int i = 0; i < 4 * ST + 4; ++i) tc::mbar_init(bar(i), bar(i) == s_free || bar(i) == p_full ? 4 : 1);
     tc::fence_barrier_init();
     tc::prefetch_tmap(&kmap);
     tc::prefetch_tmap(&vmap);
   }
-  const int part = int(blockIdx.x % unsigned(p.split)), item = int(blockIdx.x / unsigned(p.split));
+  // the first `whole` items by a block each, the others by `split`
+  const bool alone = int(blockIdx.x) < p.whole;
+  const int rest = int(blockIdx.x) - p.whole, split = alone ? 1 : p.split, part = alone ? 0 : rest % p.split;
+  const int item = alone ? int(blockIdx.x) : p.whole + rest / p.split;
   const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.Hkv, b = bh / p.Hkv;
   const int row0 = tile * kTcRows, rows = min(kTcRows, p.R * p.G - row0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -123,16 +133,40 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     tc::tmem_relinquish();
   }
   const long long n_keys = p.len ? min(max(*(const volatile long long*)(p.len + b), 0ll), p.keys) : p.keys;
-  const int all = int((n_keys + kKeys - 1) / kKeys), t0 = int((long long)all * part / p.split), n = int((long long)all * (part + 1) / p.split) - t0;
+  const int all = int((n_keys + kKeys - 1) / kKeys), t0 = int((long long)all * part / split), n = int((long long)all * (part + 1) / split) - t0;
   const int last_keys = t0 + n == all ? int(n_keys - (long long)(all - 1) * kKeys) : kKeys;  // of this block's last tile
 
+  const int kb = p.k_batch ? b : 0, kh = p.k_head ? h : 0, vb = p.v_batch ? b : 0, vh = p.v_head ? h : 0;
+  auto load_k = [&](int j) {
+    const int s = j % ST;
+    tc::mbar_arrive_expect_tx(k_full(s), L::kTile);
+    for (int x = 0; x < HALVES; ++x) tma_load_4d(base + L::kK + uint32_t(s * L::kTile + x * kKeys * 128), &kmap, x * 64, (t0 + j) * kKeys, kh, kb, k_full(s));
+  };
+  auto load_v = [&](int j) {
+    const int s = j % ST;
+    tc::mbar_arrive_expect_tx(v_full(s), L::kTile);
+    for (int x = 0; x < HALVES; ++x) tma_load_4d(base + L::kV + uint32_t(s * L::kTile + x * kKeys * 128), &vmap, x * 64, (t0 + j) * kKeys, vh, vb, v_full(s));
+  };
+  if (threadIdx.x == 0)  // the thread that made the barriers
+    for (int j = 0; j < min(n, ST); ++j) {
+      load_k(j);
+      load_v(j);
+    }
   // Q, rows of the contraction, 64 dimensions (128 bytes, chunks of 16 exchanged by the row) at a time
-  for (int i = threadIdx.x; i < kTcRows * HD / 8; i += 192) {
-    const int r = i / (HD / 8), c = i % (HD / 8), rr = row0 + r;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (r < rows) u = ld_x4(p.q + b * p.q_b + (rr / p.G) * p.q_r + (long long)(h * p.G + rr % p.G) * p.q_h + c * 8);
-    u.x ^= p.q_flip, u.y ^= p.q_flip, u.z ^= p.q_flip, u.w ^= p.q_flip;
-    tc::st_shared_v4(base + uint32_t((c / 8) * kTcRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)), u.x, u.y, u.z, u.w);
+  constexpr int kChunks = kTcRows * HD / 8, kEach = (kChunks + 191) / 192;
+  uint4 u[kEach];
+#pragma unroll
+  for (int x = 0; x < kEach; ++x) {
+    const int i = x * 192 + threadIdx.x, r = i / (HD / 8), c = i % (HD / 8), rr = row0 + r;
+    u[x] = make_uint4(0, 0, 0, 0);
+    if (r < rows) u[x] = ld_x4(p.q + b * p.q_b + (rr / p.G) * p.q_r + (long long)(h * p.G + rr % p.G) * p.q_h + c * 8);
+  }
+#pragma unroll
+  for (int x = 0; x < kEach; ++x) {
+    const int i = x * 192 + threadIdx.x, r = i / (HD / 8), c = i % (HD / 8);
+    if (i < kChunks)
+      tc::st_shared_v4(base + uint32_t((c / 8) * kTcRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)), u[x].x ^ p.q_flip, u[x].y ^ p.q_flip, u[x].z ^ p.q_flip,
+                       u[x].w ^ p.q_flip);
   }
   tc::fence_proxy_async_smem();
   tc::fence_before_sync();
@@ -143,19 +177,15 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
-      const int kb = p.k_batch ? b : 0, kh = p.k_head ? h : 0, vb = p.v_batch ? b : 0, vh = p.v_head ? h : 0;
       bool ok = true;
-      for (int j = 0; j < n && ok; ++j) {
+      for (int j = ST; j < n && ok; ++j) {
         const int s = j % ST;
         const uint32_t ph = uint32_t(j / ST) & 1u;
         ok = tc::mbar_wait(k_free(s), ph ^ 1u, p.status, 61);
         if (!ok) break;
-        tc::mbar_arrive_expect_tx(k_full(s), L::kTile);
-        for (int x = 0; x < HALVES; ++x) tma_load_4d(base + L::kK + uint32_t(s * L::kTile + x * kKeys * 128), &kmap, x * 64, (t0 + j) * kKeys, kh, kb, k_full(s));
+        load_k(j);
         ok = tc::mbar_wait(v_free(s), ph ^ 1u, p.status, 62);
-        if (!ok) break;
-        tc::mbar_arrive_expect_tx(v_full(s), L::kTile);
-        for (int x = 0; x < HALVES; ++x) tma_load_4d(base + L::kV + uint32_t(s * L::kTile + x * kKeys * 128), &vmap, x * 64, (t0 + j) * kKeys, vh, vb, v_full(s));
+        if (ok) load_v(j);
       }
       if (!ok)  // copies that are on their way still land here
         for (int s = 0; s < ST; ++s) {
@@ -176,17 +206,22 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
         for (int x = 0; x < HD / 16; ++x) {
           const uint64_t a = tc::smem_desc_sw128(base + uint32_t((x / 4) * kTcRows * 128 + (x % 4) * 32));
           const uint64_t k = tc::smem_desc_sw128(base + L::kK + uint32_t(s * L::kTile + (x / 4) * kKeys * 128 + (x % 4) * 32));
-          tc::mma_f16(tmem + uint32_t(j & 1) * kKeys, a, k, s_desc, x != 0);
+          tc::mma_f16(tmem, a, k, s_desc, x != 0);
         }
-        tc::mma_commit(s_full(j & 1));
+        tc::mma_commit(s_full);
         tc::mma_commit(k_free(s));
       }
       __syncwarp();
       return true;
     };
-    for (int j = 0; j < min(n, 2) && ok; ++j) ok = scores(j);
+    if (n > 0) ok = scores(0);
     for (int j = 0; j < n && ok; ++j) {
       const int s = j % ST;
+      if (j + 1 < n) {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(s_free, uint32_t(j) & 1u, p.status, 67));
+        if (ok) ok = scores(j + 1);
+        if (!ok) break;
+      }
       ok = __all_sync(0xffffffffu, tc::mbar_wait(v_full(s), uint32_t(j / ST) & 1u, p.status, 65));
       if (!ok) break;
       if (j == n - 1 && last_keys < kKeys) {  // values behind the last key may be anything, and their weights of zero would not silence a NaN
@@ -196,22 +231,17 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
         tc::fence_proxy_async_smem();
         __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(p_full(j & 1), uint32_t(j >> 1) & 1u, p.status, 66));
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(p_full, uint32_t(j) & 1u, p.status, 66));
       if (!ok) break;
       tc::fence_after_sync();
       if (one) {
 #pragma unroll
         for (int x = 0; x < kKeys / 16; ++x)
-          mma_f16_ts(tmem + kOut, tmem + uint32_t(j & 1) * kKeys + x * 8, smem_desc_mn_sw128(base + L::kV + uint32_t(s * L::kTile + x * 2048), kKeys * 128), o_desc,
-                     j != 0 || x != 0);
+          mma_f16_ts(tmem + kOut, tmem + kP + x * 8, smem_desc_mn_sw128(base + L::kV + uint32_t(s * L::kTile + x * 2048), kKeys * 128), o_desc, j != 0 || x != 0);
         tc::mma_commit(o_done);
         tc::mma_commit(v_free(s));
       }
       __syncwarp();
-      if (j + 2 < n) {  // its scores go where these weights were read
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(j) & 1u, p.status, 67));
-        if (ok) ok = scores(j + 2);
-      }
     }
   } else {
     const int quad = warp & 3, r = quad * 32 + lane;
@@ -219,39 +249,44 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     float m = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full(j & 1), uint32_t(j >> 1) & 1u, p.status, 68));
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full, uint32_t(j) & 1u, p.status, 68));
       if (!ok) break;
       tc::fence_after_sync();
-      uint32_t s[2][32];
-      const uint32_t at = lanes + uint32_t(j & 1) * kKeys;
-      tc::tmem_ld_32x32(at, s[0]);
-      tc::tmem_ld_32x32(at + 32, s[1]);
+      uint32_t s[kKeys / 32][32];
+#pragma unroll
+      for (int x = 0; x < kKeys / 32; ++x) tc::tmem_ld_32x32(lanes + x * 32, s[x]);
       tc::tmem_ld_wait();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(s_free);
       if (j == n - 1 && last_keys < kKeys) {
 #pragma unroll
         for (int i = 0; i < kKeys; ++i)
           if (i >= last_keys) s[i / 32][i % 32] = 0xff800000u;  // -inf
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kKeys; ++i) mx[i % 4] = fmaxf(mx[i % 4], __uint_as_float(s[i / 32][i % 32]));
-      const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+      for (int i = 0; i < kKeys; i += 2) mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], __uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
+      const float high = fmaxf(mx[0], mx[1]) * p.scale_log2;
+      // the weights' columns, and the result, are this warp's again when the product before is done
+      if (j > 0) {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(j - 1) & 1u, p.status, 69));
+        if (!ok) break;
+        tc::fence_after_sync();
+      }
       if (__any_sync(0xffffffffu, high > m + 8.f)) {
         const float now = fmaxf(m, high);
         if (j > 0) {
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(j - 1) & 1u, p.status, 69));
-          if (!ok) break;
-          tc::fence_after_sync();
           const float corr = m == now ? 1.f : ex2f(m - now);
           sum *= corr;
 #pragma unroll
-          for (int x = 0; x < HD / 32; ++x) {
-            uint32_t o[32];
-            tc::tmem_ld_32x32(lanes + kOut + x * 32, o);
+          for (int x = 0; x < HD / 16; ++x) {
+            uint32_t o[16];
+            tc::tmem_ld_32x16(lanes + kOut + x * 16, o);
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tc::tmem_st_32x32(lanes + kOut + x * 32, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st_32x16(lanes + kOut + x * 16, o);
           }
         }
         m = now;
@@ -259,33 +294,35 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
       const float ref = m == -INFINITY ? 0.f : m;
       const unsigned long long scale2 = two(p.scale_log2, p.scale_log2), less2 = two(-ref, -ref);
       unsigned long long acc[2] = {0, 0};
-      uint32_t w[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        unsigned long long x = two(__uint_as_float(s[i / 16][(2 * i) % 32]), __uint_as_float(s[i / 16][(2 * i + 1) % 32]));
-        asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(scale2), "l"(less2));
-        float lo, hi;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
-        lo = ex2f(lo);
-        hi = ex2f(hi);
-        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(two(lo, hi)));
-        w[i] = pack16<BF16>(lo, hi);
+      for (int x = 0; x < kKeys / 32; ++x) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          unsigned long long v = two(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1]));
+          asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(v) : "l"(scale2), "l"(less2));
+          float lo, hi;
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+          lo = ex2f(lo);
+          hi = ex2f(hi);
+          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(two(lo, hi)));
+          w[i] = pack16<BF16>(lo, hi);
+        }
+        tmem_st_32x16(lanes + kP + x * 16, w);
       }
       asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[0]) : "l"(acc[1]));
       float a0, a1;
       asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc[0]));
       sum += a0 + a1;
-      tc::tmem_st_32x32(at, w);
       tc::tmem_st_wait();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(p_full(j & 1));
+      if (lane == 0) tc::mbar_arrive(p_full);
     }
-    // (the product before the last one may not be done either, and its phase is the one that would be taken for the last's)
-    for (int j = max(n - 2, 0); j < n && ok; ++j) ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(j) & 1u, p.status, 70));
+    if (n > 0 && ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(n - 1) & 1u, p.status, 70));
     tc::fence_after_sync();
     const int rr = row0 + r;
-    float* to = p.parts ? p.parts + size_t(blockIdx.x) * part_floats(HD) : nullptr;
+    float* to = p.parts && !alone ? p.parts + size_t(rest) * part_floats(HD) : nullptr;
     uint16_t* out = p.out + ((size_t(b) * p.R + rr / p.G) * (p.Hkv * p.G) + h * p.G + rr % p.G) * HD;
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
@@ -317,28 +354,64 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
   if (warp == 1) tc::tmem_dealloc(tmem, 256);
 }
 
+// The results of items that several blocks share: a thread for 4 dimensions of a row, 128 a block.
+constexpr int kJoinThreads = 128;
 template <int HD, bool BF16>
-int launch_flash(const CUtensorMap& kmap, const CUtensorMap& vmap, const FlashParams& p, int64_t blocks, cudaStream_t stream) {
-  auto kern = flash_kernel<HD, BF16>;
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FlashLayout<HD>::kBytes);
-  if (rc) return rc;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float* parts, uint16_t* out, int n_parts, int first_item, int tiles, int R, int G, int Hkv) {
+  constexpr int PER = HD / 4, ROWS = kJoinThreads / PER, BLOCKS = kTcRows / ROWS;  // threads of a row, rows of a block, blocks of an item
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int at = int(blockIdx.x) / BLOCKS, item = first_item + at, bh = item / tiles, h = bh % Hkv, b = bh / Hkv;
+  const int r = (int(blockIdx.x) % BLOCKS) * ROWS + int(threadIdx.x) / PER, rr = (item % tiles) * kTcRows + r, e = (int(threadIdx.x) % PER) * 4;
+  if (rr >= R * G) return;
+  const float* from = behind_wait(parts + size_t(at) * n_parts * part_floats(HD));
+  float mx = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int x = 0; x < n_parts; ++x) mx = fmaxf(mx, from[size_t(x) * part_floats(HD) + kTcRows * HD + r * 2]);
+#pragma unroll 8
+  for (int x = 0; x < n_parts; ++x) {
+    const float* d = from + size_t(x) * part_floats(HD);
+    const float2 ml = *reinterpret_cast<const float2*>(d + kTcRows * HD + r * 2);
+    const float4 o = *reinterpret_cast<const float4*>(d + r * HD + e);
+    const float w = ml.y == 0.f ? 0.f : ex2f(ml.x - mx);  // (a sum of NaN stays one)
+    sum = fmaf(w, ml.y, sum);
+    acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  *reinterpret_cast<uint2*>(out + ((size_t(b) * R + rr / G) * (Hkv * G) + h * G + rr % G) * HD + e) =
+      make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
+}
+
+template <typename... Args>
+int launch_behind(void (*kern)(Args...), int64_t blocks, int threads, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(blocks));
-  cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = FlashLayout<HD>::kBytes;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = option(kOptNoPdl) ? 0 : 1;
-  ASRQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, kmap, vmap, p));
+  ASRQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
   return ASRQ_OK;
+}
+
+template <int HD, bool BF16>
+int launch_flash(const CUtensorMap& kmap, const CUtensorMap& vmap, const FlashParams& p, int64_t items, bool join, cudaStream_t stream) {
+  auto kern = flash_kernel<HD, BF16>;
+  int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FlashLayout<HD>::kBytes);
+  if (!rc) rc = launch_behind(kern, p.whole + (items - p.whole) * p.split, 192, FlashLayout<HD>::kBytes, stream, kmap, vmap, p);
+  if (!rc && join && p.whole < items)
+    rc = launch_behind(join_kernel<HD, BF16>, (items - p.whole) * (kTcRows * HD / 4 / kJoinThreads), kJoinThreads, 0, stream, (const float*)p.parts, p.out, p.split, p.whole, p.tiles, p.R, p.G, p.Hkv);
+  return rc;
 }
 
 }  // namespace
 
-int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, int n_parts, float* parts, void* status, int sm_count, cudaStream_t stream) {
+int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, bool join, void* status, cudaStream_t stream) {
   FlashParams p = {};
   p.q = r.q, p.out = r.out, p.len = r.len;
   p.parts = parts;
@@ -346,17 +419,19 @@ int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, int n_p
   p.q_b = r.q_b, p.q_r = r.q_r, p.q_h = r.q_h, p.keys = r.keys;
   p.R = r.R, p.G = r.G, p.Hkv = r.Hkv;
   p.tiles = (r.R * r.G + kTcRows - 1) / kTcRows;
-  p.split = n_parts;
+  p.whole = int(plan.whole);
+  p.split = plan.split;
   p.scale_log2 = r.scale_log2 < 0.f ? -r.scale_log2 : r.scale_log2;
   p.q_flip = r.scale_log2 < 0.f ? 0x80008000u : 0u;
   p.k_batch = r.k_b != 0, p.v_batch = r.v_b != 0, p.k_head = r.k_h != 0, p.v_head = r.v_h != 0;
+  const uint32_t keys = hd == 64 ? FlashLayout<64>::kKeys : FlashLayout<128>::kKeys;
   CUtensorMap kmap, vmap;
-  int rc = make_tmap_4d(&kmap, r.k, bf16, hd, uint64_t(r.keys), r.k_h ? r.Hkv : 1, r.k_b ? uint64_t(B) : 1, r.k_t, r.k_h, r.k_b, 64, kKeys);
-  if (!rc) rc = make_tmap_4d(&vmap, r.v, bf16, hd, uint64_t(r.keys), r.v_h ? r.Hkv : 1, r.v_b ? uint64_t(B) : 1, r.v_t, r.v_h, r.v_b, 64, kKeys);
+  int rc = make_tmap_4d(&kmap, r.k, bf16, hd, uint64_t(r.keys), r.k_h ? r.Hkv : 1, r.k_b ? uint64_t(B) : 1, r.k_t, r.k_h, r.k_b, 64, keys);
+  if (!rc) rc = make_tmap_4d(&vmap, r.v, bf16, hd, uint64_t(r.keys), r.v_h ? r.Hkv : 1, r.v_b ? uint64_t(B) : 1, r.v_t, r.v_h, r.v_b, 64, keys);
   if (rc) return rc;
-  const int64_t blocks = B * p.Hkv * p.tiles * n_parts;
-  if (hd == 64) return bf16 ? launch_flash<64, true>(kmap, vmap, p, blocks, stream) : launch_flash<64, false>(kmap, vmap, p, blocks, stream);
-  return bf16 ? launch_flash<128, true>(kmap, vmap, p, blocks, stream) : launch_flash<128, false>(kmap, vmap, p, blocks, stream);
+  const int64_t items = B * p.Hkv * p.tiles;
+  if (hd == 64) return bf16 ? launch_flash<64, true>(kmap, vmap, p, items, join, stream) : launch_flash<64, false>(kmap, vmap, p, items, join, stream);
+  return bf16 ? launch_flash<128, true>(kmap, vmap, p, items, join, stream) : launch_flash<128, false>(kmap, vmap, p, items, join, stream);
 }
 
 }  // namespace asrq
