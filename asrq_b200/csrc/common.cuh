@@ -44,6 +44,7 @@ enum Option {
   kOptTcPairRelease, // CTA-pair prefill: 1 = release-ordered cross-CTA arrivals (one per dequant warp), 0 = relaxed
   kOptW4a4Bt,        // W4A4 GEMM: token-tile width (0 auto)
   kOptW4a4Pair,      // W4A4 GEMM: -1 auto, 0 one CTA per tile, 1 CTA pairs
+  kOptRowsKernel,    // attention over shared keys: 0 auto, 1 the row kernel, 2 the tensor-core kernel wherever it can run
   kOptTrace,         // builds with -DASRQ_TRACE only: 1 records pipeline clock marks into the workspace
   kOptTraceBlock,    // builds with -DASRQ_TRACE only: which block records
   kOptCount

@@ -561,7 +561,8 @@ TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys
   const int64_t rows = R * G, tiles = (rows + kTcRows - 1) / kTcRows, items = B * n_kv_heads * tiles, step = hd == 64 ? 96 : 64;
   const int64_t key_tiles = (keys + step - 1) / step, slots = 2 * sm_count;
   const bool own = keys2 > 0;
-  if (rows <= 16 || keys < 64) return {0, 0};
+  const int forced = option(kOptRowsKernel);
+  if (keys == 0 || forced == 1 || (forced != 2 && (rows <= 16 || keys < 64))) return {0, 0};
   const int64_t whole = own ? 0 : items / slots * slots, rest = items - whole, first = whole / slots * (key_tiles + 3);
   TcPlan plan = {own ? 0 : items, own ? 0 : 1};
   int64_t least = rest == 0 ? 0 : own ? INT64_MAX : key_tiles + 3;
@@ -572,6 +573,7 @@ TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys
       plan = {whole, s};
     }
   }
+  if (forced == 2) return plan;
   double us = 1.3 * double(first + least);
   if (own) us += rows_estimate(B, R, G, n_kv_heads, hd, 0, keys2, true, sm_count);
   return us < rows_estimate(B, R, G, n_kv_heads, hd, keys, keys2, false, sm_count) ? plan : TcPlan{0, 0};
@@ -617,7 +619,8 @@ int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_
   TcPlan plan = {0, 0};
   int rc = allow_all();
   if (rc) return rc;
-  if (status && ((ks[2] && vs[2]) || keys == 1)) plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
+  // (the tensor-core kernel copies keys at a stride, and hides scores before it scales them)
+  if (status && ((ks[2] && vs[2]) || keys == 1) && p.scale_log2 != 0.f) plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
   if (plan.split > 0) {
     const size_t need = part_bytes(B, R, p.G, n_kv_heads, hd, plan);
     const bool kept = need == 0 || (scratch && scratch_bytes >= need);

@@ -95,6 +95,11 @@ __device__ __forceinline__ unsigned long long two(float a, float b) {
   return v;
 }
 
+// Most waits find their phase over: a test first, which unlike try_wait never suspends the warp.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, unsigned* status, unsigned site) {
+  return tc::mbar_test_wait(bar, parity) || tc::mbar_wait(bar, parity, status, site);
+}
+
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(192, 2)
 flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FlashParams p) {
@@ -127,13 +132,28 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
   const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.Hkv, b = bh / p.Hkv;
   const int row0 = tile * kTcRows, rows = min(kTcRows, p.R * p.G - row0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  // Tensor memory only now, and the next kernel only behind it: a block that held it while it waits could keep it from one that it waits for.
+  // Q on its way first: all warps but the one that starts the copies
+  constexpr int kChunks = kTcRows * HD / 8, kEach = (kChunks + 159) / 160;
+  uint4 u[kEach];
+  const uint16_t* q = p.q + b * p.q_b + (long long)(h * p.G) * p.q_h;
+  const int q0 = int(threadIdx.x) - 32;
+#pragma unroll
+  for (int x = 0; x < kEach; ++x) {
+    const int i = x * 160 + q0, r = i / (HD / 8), c = i % (HD / 8), rr = row0 + r;
+    const int token = p.G == 1 ? rr : rr / p.G;
+    u[x] = make_uint4(0, 0, 0, 0);
+    if (q0 >= 0 && r < rows) u[x] = ld_x4(q + token * p.q_r + (long long)(rr - token * p.G) * p.q_h + c * 8);
+  }
+  const long long n_keys = p.len ? min(max(*(const volatile long long*)(p.len + b), 0ll), p.keys) : p.keys;
+  // (fewer than 2^25 tiles, at most 64 parts)
+  const int all = int((n_keys + kKeys - 1) / kKeys), t0 = int(unsigned(all) * unsigned(part) / unsigned(split));
+  const int n = int(unsigned(all) * unsigned(part + 1) / unsigned(split)) - t0;
+  // Tensor memory only behind the wait, and the next kernel only behind it: a block that held it while it waits could keep it from one that it
+  // waits for.
   if (warp == 1) {
     tc::tmem_alloc(tc::smem_u32(tmem_at), 256);
     tc::tmem_relinquish();
   }
-  const long long n_keys = p.len ? min(max(*(const volatile long long*)(p.len + b), 0ll), p.keys) : p.keys;
-  const int all = int((n_keys + kKeys - 1) / kKeys), t0 = int((long long)all * part / split), n = int((long long)all * (part + 1) / split) - t0;
   const int last_keys = t0 + n == all ? int(n_keys - (long long)(all - 1) * kKeys) : kKeys;  // of this block's last tile
 
   const int kb = p.k_batch ? b : 0, kh = p.k_head ? h : 0, vb = p.v_batch ? b : 0, vh = p.v_head ? h : 0;
@@ -153,18 +173,10 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
       load_v(j);
     }
   // Q, rows of the contraction, 64 dimensions (128 bytes, chunks of 16 exchanged by the row) at a time
-  constexpr int kChunks = kTcRows * HD / 8, kEach = (kChunks + 191) / 192;
-  uint4 u[kEach];
 #pragma unroll
   for (int x = 0; x < kEach; ++x) {
-    const int i = x * 192 + threadIdx.x, r = i / (HD / 8), c = i % (HD / 8), rr = row0 + r;
-    u[x] = make_uint4(0, 0, 0, 0);
-    if (r < rows) u[x] = ld_x4(p.q + b * p.q_b + (rr / p.G) * p.q_r + (long long)(h * p.G + rr % p.G) * p.q_h + c * 8);
-  }
-#pragma unroll
-  for (int x = 0; x < kEach; ++x) {
-    const int i = x * 192 + threadIdx.x, r = i / (HD / 8), c = i % (HD / 8);
-    if (i < kChunks)
+    const int i = x * 160 + q0, r = i / (HD / 8), c = i % (HD / 8);
+    if (q0 >= 0 && i < kChunks)
       tc::st_shared_v4(base + uint32_t((c / 8) * kTcRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)), u[x].x ^ p.q_flip, u[x].y ^ p.q_flip, u[x].z ^ p.q_flip,
                        u[x].w ^ p.q_flip);
   }
@@ -181,16 +193,16 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
       for (int j = ST; j < n && ok; ++j) {
         const int s = j % ST;
         const uint32_t ph = uint32_t(j / ST) & 1u;
-        ok = tc::mbar_wait(k_free(s), ph ^ 1u, p.status, 61);
+        ok = wait(k_free(s), ph ^ 1u, p.status, 61);
         if (!ok) break;
         load_k(j);
-        ok = tc::mbar_wait(v_free(s), ph ^ 1u, p.status, 62);
+        ok = wait(v_free(s), ph ^ 1u, p.status, 62);
         if (ok) load_v(j);
       }
       if (!ok)  // copies that are on their way still land here
         for (int s = 0; s < ST; ++s) {
-          tc::mbar_wait(k_full(s), 0, p.status, 63);
-          tc::mbar_wait(v_full(s), 0, p.status, 63);
+          wait(k_full(s), 0, p.status, 63);
+          wait(v_full(s), 0, p.status, 63);
         }
     }
   } else if (warp == 1) {
@@ -199,7 +211,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     bool ok = true;
     auto scores = [&](int j) {  // of tile j
       const int s = j % ST;
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(k_full(s), uint32_t(j / ST) & 1u, p.status, 64))) return false;
+      if (!__all_sync(0xffffffffu, wait(k_full(s), uint32_t(j / ST) & 1u, p.status, 64))) return false;
       tc::fence_after_sync();
       if (one) {
 #pragma unroll
@@ -218,11 +230,11 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     for (int j = 0; j < n && ok; ++j) {
       const int s = j % ST;
       if (j + 1 < n) {
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(s_free, uint32_t(j) & 1u, p.status, 67));
+        ok = __all_sync(0xffffffffu, wait(s_free, uint32_t(j) & 1u, p.status, 67));
         if (ok) ok = scores(j + 1);
         if (!ok) break;
       }
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(v_full(s), uint32_t(j / ST) & 1u, p.status, 65));
+      ok = __all_sync(0xffffffffu, wait(v_full(s), uint32_t(j / ST) & 1u, p.status, 65));
       if (!ok) break;
       if (j == n - 1 && last_keys < kKeys) {  // values behind the last key may be anything, and their weights of zero would not silence a NaN
         const uint32_t v = base + L::kV + uint32_t(s * L::kTile);
@@ -231,7 +243,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
         tc::fence_proxy_async_smem();
         __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(p_full, uint32_t(j) & 1u, p.status, 66));
+      ok = __all_sync(0xffffffffu, wait(p_full, uint32_t(j) & 1u, p.status, 66));
       if (!ok) break;
       tc::fence_after_sync();
       if (one) {
@@ -249,7 +261,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     float m = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(s_full, uint32_t(j) & 1u, p.status, 68));
+      ok = __all_sync(0xffffffffu, wait(s_full, uint32_t(j) & 1u, p.status, 68));
       if (!ok) break;
       tc::fence_after_sync();
       uint32_t s[kKeys / 32][32];
@@ -270,7 +282,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
       const float high = fmaxf(mx[0], mx[1]) * p.scale_log2;
       // the weights' columns, and the result, are this warp's again when the product before is done
       if (j > 0) {
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(j - 1) & 1u, p.status, 69));
+        ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(j - 1) & 1u, p.status, 69));
         if (!ok) break;
         tc::fence_after_sync();
       }
@@ -319,7 +331,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(p_full);
     }
-    if (n > 0 && ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, uint32_t(n - 1) & 1u, p.status, 70));
+    if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(n - 1) & 1u, p.status, 70));
     tc::fence_after_sync();
     const int rr = row0 + r;
     float* to = p.parts && !alone ? p.parts + size_t(rest) * part_floats(HD) : nullptr;

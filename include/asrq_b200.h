@@ -497,6 +497,8 @@ int asrq_w4a4_gemm_f8(const uint8_t* a8, const float* sa, const uint8_t* w8, con
  *                         unpacks the weights once per call, where the call has scratch for them
  *   tc_pair_release (0)   CTA-pair prefill kernel: 1 = release/acquire at cluster scope on the
  *                         cross-CTA "operand written" hand-off (slower), 0 = relaxed arrival
+ *   rows_kernel (0)       asrq_cross_attention, asrq_prefix_attention: 0 = by estimated time, 1 = the row kernel,
+ *                         2 = the tensor-core kernel wherever it can run
  *   trace (0), trace_block (0)     only in builds with -DASRQ_TRACE: pipeline clock marks
  * Returns ASRQ_ERR_SHAPE for an unknown name.  No counterpart in the reference.
  */

@@ -3,10 +3,20 @@ import pytest
 import torch
 
 import asrq_b200
+from asrq_b200 import _lib
 from tests.beam_util import check_rows
 
 DEV = "cuda"
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["row kernel", "tensor cores"])
+def kernel(request):
+    """Every test on both kernels, whatever the estimates would choose."""
+    _lib.set_option("rows_kernel", 1 if request.param == "row kernel" else 2)
+    yield
+    _lib.set_option("rows_kernel", 0)
+    asrq_b200.check_status()
 
 
 def _rnd(seed, *shape, dtype=torch.float16, std=1.0):
