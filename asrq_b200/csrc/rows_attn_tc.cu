@@ -9,7 +9,8 @@
 // The reference exponent m of a row moves only when its maximum has grown by more than 8 (a weight stays below 2^8, a sum in 32 bits has
 // room for that): O is scaled at the first tiles and hardly ever after.
 //
-// Bound: at 64 dimensions the exponentials, 16 a cycle and SM; at 128 these and the memory's bytes where few rows share many keys.
+// Bound: at 64 dimensions the exponentials, 16 a cycle and SM, of which every fourth pair goes to the multipliers instead; at 128 these and the
+// memory's bytes where few rows share many keys.
 #include "rows_attn.cuh"
 
 namespace asrq {
@@ -93,6 +94,31 @@ __device__ __forceinline__ unsigned long long two(float a, float b) {
   unsigned long long v;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
   return v;
+}
+
+// 2^x of a pair without the exponential unit, x at most 100 and below -126 as -126: x = i + f with a whole i and f within a half (adding 1.5 * 2^23
+// leaves i in the low bits), 2^f by the polynomial of degree 4 with the least relative error there (Remez' exchange: 2.6e-6), times 2^i.
+__device__ __forceinline__ unsigned long long ex2_poly(unsigned long long x) {
+  constexpr float kShift = 12582912.f + 127.f;  // the exponent's bias with it
+  constexpr float c0 = 0.9999992847442627f, c1 = 0.6931217908859253f, c2 = 0.240247443318367f, c3 = 0.05591785907745361f, c4 = 0.009570102207362652f;
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(lo));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(hi));
+  x = two(lo, hi);
+  unsigned long long i = x, f = x, y = two(c4, c4);
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(i) : "l"(two(kShift, kShift)));
+  unsigned long long whole = i;
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(whole) : "l"(two(-kShift, -kShift)));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(f) : "l"(whole), "l"(two(-1.f, -1.f)));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(f), "l"(two(c3, c3)));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(f), "l"(two(c2, c2)));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(f), "l"(two(c1, c1)));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(f), "l"(two(c0, c0)));
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(i));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(two(__uint_as_float(a << 23), __uint_as_float(b << 23))));
+  return y;
 }
 
 // Most waits find their phase over: a test first, which unlike try_wait never suspends the warp.
@@ -313,11 +339,16 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
         for (int i = 0; i < 16; ++i) {
           unsigned long long v = two(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1]));
           asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(v) : "l"(scale2), "l"(less2));
+          if (i % 4 == 3) {
+            v = ex2_poly(v);
+          } else {
+            float lo, hi;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+            v = two(ex2f(lo), ex2f(hi));
+          }
+          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(v));
           float lo, hi;
           asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-          lo = ex2f(lo);
-          hi = ex2f(hi);
-          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(two(lo, hi)));
           w[i] = pack16<BF16>(lo, hi);
         }
         tmem_st_32x16(lanes + kP + x * 16, w);
@@ -333,6 +364,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     }
     if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(n - 1) & 1u, p.status, 70));
     tc::fence_after_sync();
+    if (m == -INFINITY && sum == sum) sum = 0.f;  // nothing above -inf
     const int rr = row0 + r;
     float* to = p.parts && !alone ? p.parts + size_t(rest) * part_floats(HD) : nullptr;
     uint16_t* out = p.out + ((size_t(b) * p.R + rr / p.G) * (p.Hkv * p.G) + h * p.G + rr % p.G) * HD;
