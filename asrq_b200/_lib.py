@@ -83,7 +83,7 @@ SIGNATURES = {
     "asrq_decode_grouped_attention": (c_int, [c_void_p] * 9 + [c_int64, c_int, c_int, c_int, c_int64, ctypes.c_float, ctypes.c_float, c_int,
                                               c_void_p]),
     "asrq_beam_select": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4 + [c_int64] * 4 + [c_int, c_void_p]),
-    "asrq_beam_reorder": (c_int, [c_void_p] * 3 + [c_int64] * 7 + [c_void_p]),
+    "asrq_beam_reorder": (c_int, [c_void_p] * 3 + [c_int64] * 7 + [c_void_p, c_size_t, c_void_p]),
     "asrq_cross_attention": (c_int, [c_void_p, _I64P] * 3 + [c_void_p] * 2 + [c_int64] * 2 + [c_int] * 3 + [c_int64, ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
     "asrq_rows_attention_scratch_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int64]),
     "asrq_prefix_attention": (c_int, [c_void_p, _I64P] * 3 + [c_void_p] + [c_void_p, _I64P] * 2 + [c_void_p, c_int64, c_void_p] + [c_int64] * 2 + [c_int] * 3 +

@@ -77,8 +77,10 @@ def beam_reorder(cache: torch.Tensor, parents: torch.Tensor, length) -> torch.Te
         return cache
     parents = parents.contiguous()
     with _on_device(cache.device):
+        ws = _workspace(cache.device, _lib.STATUS_BYTES)
         _lib.call("asrq_beam_reorder", cache.data_ptr(), parents.data_ptr(), length.data_ptr() if on_dev else None, 0 if on_dev else int(length), L,
-                  parents.shape[0], parents.shape[1], H, M, hd * cache.element_size(), torch.cuda.current_stream(cache.device).cuda_stream)
+                  parents.shape[0], parents.shape[1], H, M, hd * cache.element_size(), ws.data_ptr(), ws.numel(),
+                  torch.cuda.current_stream(cache.device).cuda_stream)
     return cache
 
 

@@ -62,7 +62,7 @@ int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores,
                 long long* parents, long long* tokens, uint8_t* out_finished, int64_t B, int64_t K, int64_t V, int64_t n, int dtype, int sm_count,
                 cudaStream_t stream);
 int beam_reorder(void* cache, const long long* parents, const long long* length_dev, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
-                 int64_t max_len, int64_t pos_bytes, cudaStream_t stream);
+                 int64_t max_len, int64_t pos_bytes, void* status, int sm_count, cudaStream_t stream);
 int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
                    const void* k2, const int64_t* k2s, const void* v2, const int64_t* v2s, const long long* lengths2, bool lengths2_many, void* out,
                    int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, float scale, int dtype, void* status, void* scratch,
@@ -759,7 +759,7 @@ int asrq_beam_select(const void* logits, int64_t utterance_stride, int64_t beam_
 }
 
 int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length_device, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
-                      int64_t max_len, int64_t position_bytes, void* stream) {
+                      int64_t max_len, int64_t position_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   last_error().clear();
   if (!cache || !parents) return fail(ASRQ_ERR_NULL, "asrq_beam_reorder: cache and parents must not be NULL");
   if (L < 0 || B < 0 || K <= 0 || heads <= 0 || max_len <= 0 || position_bytes <= 0 || position_bytes % 16 || position_bytes > (1 << 20) ||
@@ -768,12 +768,13 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
                 (long long)B, (long long)K, (long long)heads, (long long)max_len, (long long)position_bytes);
   if (K > 32) return fail(ASRQ_ERR_LIMIT, "asrq_beam_reorder: K=%lld (at most 32)", (long long)K);
   if (!aligned16(cache)) return fail(ASRQ_ERR_ALIGN, "asrq_beam_reorder: cache must be 16-byte aligned");
+  if (!workspace || workspace_bytes < kStatusBytes) return fail(ASRQ_ERR_WORKSPACE, "asrq_beam_reorder: workspace");
   const DeviceFacts* f;
   int rc;
   if ((rc = device_facts(&f))) return rc;
   if (L == 0 || B == 0 || K == 1) return ASRQ_OK;
   return beam_reorder(cache, reinterpret_cast<const long long*>(parents), reinterpret_cast<const long long*>(length_device), length, L, B, K, heads, max_len,
-                      position_bytes, static_cast<cudaStream_t>(stream));
+                      position_bytes, workspace, f->sm_count, static_cast<cudaStream_t>(stream));
 }
 
 namespace {

@@ -507,41 +507,113 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
   }
 }
 
-// One block per (layer and kind, utterance, head): a thread takes a 16-byte vector of one position in all beams, reads what moves
-// and writes it, so no thread reads what another writes.
-template <int MAXK>
-__global__ void __launch_bounds__(256)
-beam_reorder_kernel(uint4* __restrict__ cache, const long long* parents, const long long* length_dev, long long length, int K, int heads,
-                    long long row_vecs, long long head_vecs, int pos_vecs, long long max_len, int B) {
-  __shared__ int from[MAXK];
-  __shared__ int moves;
+// A run is what one (layer and kind, utterance, head) has to move in each of its beams: `length` positions, contiguous.  A warp a block, three an SM,
+// each with its share of the runs in order; a chunk of a run is copied from every beam that another takes over into shared memory, and
+// from there to every beam that takes one over, so each is read once, and all of it is read before any of it is written.  Copies and
+// stores are bulk copies, four chunks under way.  (Loads and stores of threads ran at 4.5 to 5.8 TB/s of the row sizes tried, by block size
+// and cache operator without a rule; this at 5.6 to 5.8 everywhere.)
+constexpr int kMoveStages = 4, kMoveBytes = 16384, kMoveBlocks = 3;
+
+struct ReorderParams {
+  char* cache;
+  const long long *parents, *length_dev;
+  long long length, max_len, row_bytes, head_bytes, pos_bytes;
+  int K, heads, B, L;
+  unsigned* status;
+};
+
+__global__ void __launch_bounds__(32) beam_reorder_kernel(const ReorderParams p) {
+  extern __shared__ __align__(128) uint8_t move_smem[];
+  __shared__ __align__(8) unsigned long long full_bar[kMoveStages];
+  const int lane = threadIdx.x;
+  if (lane == 0) {
+    for (int s = 0; s < kMoveStages; ++s) tc::mbar_init(tc::smem_u32(&full_bar[s]), 1);
+    tc::fence_barrier_init();
+  }
+  __syncwarp();
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int h = blockIdx.x % heads;
-  const long long lb = blockIdx.x / heads;
-  const int b = int(lb % B);
-  if (threadIdx.x == 0) moves = 0;
-  __syncthreads();
-  if (threadIdx.x < MAXK) {
-    const int k = threadIdx.x;
-    long long f = k < K ? *(const volatile long long*)(parents + (long long)b * K + k) : k;
-    if (f < 0 || f >= K) f = k;  // no such beam: stays as it is
-    from[k] = int(f);
-    if (f != k) moves = 1;
+  const long long length = p.length_dev ? *(const volatile long long*)p.length_dev : p.length;
+  const long long run = min(max(length, 0ll), p.max_len) * p.pos_bytes;
+  const int runs_of = p.L * p.heads, items = runs_of * p.B;  // of an utterance; of all, utterance by utterance
+  const int share = (items + int(gridDim.x) - 1) / int(gridDim.x), end = min(items, (int(blockIdx.x) + 1) * share);
+  struct Cursor {
+    int item, b;         // run; the utterance that what follows is of
+    long long off;       // in the run
+    int parent, chunk;   // this lane's beam's parent; bytes copied from a beam at a time
+    unsigned moves, from;  // beams that take another over; beams that are taken over
+  };
+  auto find = [&](Cursor& c) {  // to the next run with something to move
+    while (c.item < end && run > 0) {
+      const int b = c.item / runs_of;
+      if (b != c.b) {
+        c.b = b;
+        long long f = lane < p.K ? *(const volatile long long*)(p.parents + (long long)b * p.K + lane) : lane;
+        if (f < 0 || f >= p.K) f = lane;  // no such beam: stays as it is
+        c.parent = int(f);
+        c.moves = __ballot_sync(0xffffffffu, c.parent != lane);
+        c.from = __reduce_or_sync(0xffffffffu, c.parent != lane ? 1u << c.parent : 0u);
+        c.chunk = (kMoveBytes / max(1, __popc(c.from))) & ~127;
+      }
+      if (c.moves) return true;
+      c.item = min(end, (b + 1) * runs_of);
+    }
+    return false;
+  };
+  auto step = [&](Cursor& c) {
+    c.off += c.chunk;
+    if (c.off >= run) {
+      c.off = 0;
+      ++c.item;
+    }
+  };
+  auto place = [&](const Cursor& c) {
+    const int x = c.item - c.b * runs_of, l = x / p.heads;
+    return p.cache + ((long long)l * p.B + c.b) * p.K * p.row_bytes + (x - l * p.heads) * p.head_bytes + c.off;
+  };
+  auto bytes_of = [&](const Cursor& c) { return uint32_t(min((long long)c.chunk, run - c.off)); };
+  Cursor in = {int(blockIdx.x) * share, -1, 0, 0, 0, 0, 0}, out = in;
+  int started = 0;
+  auto start = [&]() {  // the next chunk's copies
+    const int s = started % kMoveStages;
+    const uint32_t bytes = bytes_of(in), bar = tc::smem_u32(&full_bar[s]), to = tc::smem_u32(move_smem) + uint32_t(s * kMoveBytes);
+    if (lane == 0) {
+      tc::mbar_arrive_expect_tx(bar, bytes * __popc(in.from));
+      const char* at = place(in);
+      int slot = 0;
+      for (unsigned m = in.from; m; m &= m - 1, ++slot)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to + uint32_t(slot * in.chunk)),
+                     "l"(at + (__ffs(m) - 1) * p.row_bytes), "r"(bytes), "r"(bar)
+                     : "memory");
+    }
+    step(in);
+    ++started;
+  };
+  for (int s = 0; s < kMoveStages - 1 && find(in); ++s) start();
+  int done = 0;
+  bool ok = true;
+  for (; ok && find(out); ++done) {
+    const int s = done % kMoveStages;
+    ok = __all_sync(0xffffffffu, tc::mbar_wait(tc::smem_u32(&full_bar[s]), uint32_t(done / kMoveStages) & 1u, p.status, 81));
+    if (!ok) break;
+    const uint32_t bytes = bytes_of(out), from = tc::smem_u32(move_smem) + uint32_t(s * kMoveBytes);
+    char* at = place(out);
+    for (unsigned m = out.moves; m; m &= m - 1) {
+      const int k = __ffs(m) - 1, f = __shfl_sync(0xffffffffu, out.parent, k), slot = __popc(out.from & ((1u << f) - 1u));
+      if (lane == 0)
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(at + k * p.row_bytes), "r"(from + uint32_t(slot * out.chunk)), "r"(bytes)
+                     : "memory");
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    step(out);
+    if (find(in)) {  // into the stage that the chunk before this one has left
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      __syncwarp();
+      start();
+    }
   }
-  __syncthreads();
-  if (!moves) return;
-  const long long len = min(max(length_dev ? *(const volatile long long*)length_dev : length, 0ll), max_len);
-  uint4* base = cache + (lb * K * heads + h) * head_vecs;
-  const long long n = len * pos_vecs;
-  for (long long i = threadIdx.x; i < n; i += 256) {
-    uint4 v[MAXK];
-#pragma unroll
-    for (int k = 0; k < MAXK; ++k)
-      if (from[k] != k) v[k] = base[from[k] * row_vecs + i];
-#pragma unroll
-    for (int k = 0; k < MAXK; ++k)
-      if (from[k] != k) base[k * row_vecs + i] = v[k];
-  }
+  for (; done < started && !ok; ++done)  // copies that are on their way still land here
+    tc::mbar_wait(tc::smem_u32(&full_bar[done % kMoveStages]), uint32_t(done / kMoveStages) & 1u, p.status, 82);
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 }  // namespace
@@ -620,21 +692,31 @@ int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores,
 }
 
 int beam_reorder(void* cache, const long long* parents, const long long* length_dev, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
-                 int64_t max_len, int64_t pos_bytes, cudaStream_t stream) {
-  auto kern = K <= 8 ? beam_reorder_kernel<8> : K <= 16 ? beam_reorder_kernel<16> : beam_reorder_kernel<32>;
-  const int pos_vecs = int(pos_bytes / 16);
-  const long long head_vecs = max_len * pos_vecs;
+                 int64_t max_len, int64_t pos_bytes, void* status, int sm_count, cudaStream_t stream) {
+  ReorderParams p = {};
+  p.cache = static_cast<char*>(cache);
+  p.parents = parents;
+  p.length_dev = length_dev;
+  p.length = length;
+  p.max_len = max_len;
+  p.pos_bytes = pos_bytes;
+  p.head_bytes = max_len * pos_bytes;
+  p.row_bytes = heads * p.head_bytes;
+  p.K = int(K), p.heads = int(heads), p.B = int(B), p.L = int(L);
+  p.status = static_cast<unsigned*>(status);
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(beam_reorder_kernel), kMoveStages * kMoveBytes);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(L * B * heads));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(int64_t(kMoveBlocks) * sm_count, L * B * heads)));
+  cfg.blockDim = dim3(32);
+  cfg.dynamicSmemBytes = kMoveStages * kMoveBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = option(kOptNoPdl) ? 0 : 1;
-  ASRQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<uint4*>(cache), parents, length_dev, (long long)length, int(K), int(heads),
-                                   heads * head_vecs, head_vecs, pos_vecs, (long long)max_len, int(B)));
+  ASRQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, beam_reorder_kernel, p));
   return ASRQ_OK;
 }
 

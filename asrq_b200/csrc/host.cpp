@@ -387,12 +387,17 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (!len || len->device() != x->device() || len->scalar_type() != at::kLong || len->numel() != 1) Py_RETURN_NONE;
   }
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(x->device().index()).stream();
+  Held ws;
+  if (!workspace(x->device().index(), stream, 256, &ws)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;  // the Python path makes it
+  }
   int rc;
   {
     Unlocked unlocked;
     g_calls.fetch_add(1, std::memory_order_relaxed);
     rc = asrq_beam_reorder(x->data_ptr(), static_cast<const int64_t*>(p->data_ptr()), len ? static_cast<const int64_t*>(len->data_ptr()) : nullptr, length, x->size(0),
-                           p->size(0), p->size(1), x->size(2), x->size(3), x->size(4) * x->element_size(), stream);
+                           p->size(0), p->size(1), x->size(2), x->size(3), x->size(4) * x->element_size(), ws->data_ptr(), size_t(ws->numel()), stream);
   }
   if (rc) return failed("asrq_beam_reorder", rc);
   Py_RETURN_TRUE;

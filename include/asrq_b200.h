@@ -326,11 +326,12 @@ int asrq_beam_select(const void* logits, int64_t utterance_stride, int64_t beam_
  * h < heads and the positions t < length, in place; positions from `length` on stay as they are.  cache: L x (B * K) x heads x max_len
  * positions of position_bytes (a multiple of 16), any type, 16-byte aligned.  parents: B x K; a parent outside 0..K-1 leaves its beam as it is.
  * The length is read from length_device when that is not NULL and is the argument otherwise, and is cut to 0..max_len.  K at most 32.
+ * workspace: at least 256 bytes, the status block of any workspace (the kernel's waits are bounded; asrq_check_status).
  * A kernel that reads the cache ahead of the stream dependency (asrq_decode_self_attention_settled,
  * asrq_decode_grouped_attention) needs an ordinary kernel or copy between this call and its own.
  */
 int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length_device, int64_t length, int64_t L, int64_t B, int64_t K, int64_t heads,
-                      int64_t max_len, int64_t position_bytes, void* stream);
+                      int64_t max_len, int64_t position_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Attention of R query rows of every utterance (the beams of a step, the tokens of a prompt) over its encoder states:

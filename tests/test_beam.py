@@ -36,13 +36,13 @@ def test_select_refusals(kw, code):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(cache=None), -1), (dict(parents=None), -1), (dict(K=0), -2), (dict(bytes=24), -2), (dict(bytes=0), -2), (dict(L=-1), -2), (dict(heads=0), -2),
-    (dict(max_len=0), -2), (dict(K=33), -8), (dict(odd=2), -3),
+    (dict(max_len=0), -2), (dict(K=33), -8), (dict(odd=2), -3), (dict(ws=None), -4), (dict(ws_bytes=255), -4),
 ])
 def test_reorder_refusals(kw, code):
     keep, p = _ptr()
-    a = dict(cache=p, parents=p, L=1, B=1, K=2, heads=1, max_len=4, bytes=16, odd=0)
+    a = dict(cache=p, parents=p, L=1, B=1, K=2, heads=1, max_len=4, bytes=16, odd=0, ws=p, ws_bytes=256)
     a.update(kw)
-    rc = _lib.load().asrq_beam_reorder(a["cache"] and a["cache"] + a["odd"], a["parents"], None, 2, a["L"], a["B"], a["K"], a["heads"], a["max_len"], a["bytes"], None)
+    rc = _lib.load().asrq_beam_reorder(a["cache"] and a["cache"] + a["odd"], a["parents"], None, 2, a["L"], a["B"], a["K"], a["heads"], a["max_len"], a["bytes"], a["ws"], a["ws_bytes"], None)
     assert rc == code and "asrq_beam_reorder" in _lib.last_error()
 
 
