@@ -29,7 +29,6 @@ namespace {
 
 constexpr int kRowsWarps = 8;
 constexpr int kMaxSplit = 16;  // blocks of a cluster
-constexpr int kMaxParts = 64;  // of the tensor-core kernel
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -98,8 +97,6 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
   float* gathered = part + nw * kPart;       // ROWS x HD: this block's share of the result, from every block of the cluster
   float* stats = gathered + ROWS * HD;       // blocks x ROWS x 2: their maxima and sums
   float* total_of = stats + 2 * kMaxSplit * ROWS;  // ROWS x 2: the block's (then the cluster's) maximum and sum
-  float* part_w = total_of + 2 * ROWS;       // ROWS x kMaxParts: sums, then weights
-  float* part_m = part_w + ROWS * kMaxParts;
   uint32_t rank, nsplit;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nsplit));
@@ -108,11 +105,9 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
   const int item = int(blockIdx.x / nsplit);
   const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.Hkv, b = bh / p.Hkv;
   const int row0 = tile * ROWS, rows = min(ROWS, p.R * p.G - row0);
-  // Behind the tensor-core kernel of the same call only its parts are waited for: it has itself waited for all before it.
-  if (!p.parts) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  }
+  // Behind the tensor-core kernel of the same call, which has itself waited for all before it, nothing is waited for until the end.
+  if (!p.parts) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the row tile's chunks: the shared keys', then those of each of its rows' own keys, lane i holding the i-th's
   const long long n1 = p.len ? min(max(*(const volatile long long*)(p.len + b), 0ll), p.keys) : p.keys;
@@ -357,23 +352,8 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
         d[HD + 1] = l[mt][half];
       }
     }
-  // What the tensor-core kernel left, every block of the cluster its share of the parts.
-  const int n_parts = p.parts ? (p.n_parts - int(rank) + int(nsplit) - 1) / int(nsplit) : 0;
-  const float* from = nullptr;
-  if (p.parts) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // (a row tile does not cross a tile of 128)
-    from = behind_wait(p.parts + ((size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + row0 / kTcRows) * p.n_parts + rank) * part_floats(HD));
-    for (int i = threadIdx.x; i < rows * n_parts; i += blockDim.x) {
-      const int r = i / n_parts, x = i % n_parts;
-      const float2 ml = *reinterpret_cast<const float2*>(from + size_t(x) * nsplit * part_floats(HD) + kTcRows * HD + (row0 % kTcRows + r) * 2);
-      part_m[r * kMaxParts + x] = ml.x;
-      part_w[r * kMaxParts + x] = ml.y;
-    }
-  }
   __syncthreads();
-  // a warp a row: its maximum and sum over warps and parts, and their weights (a sum of NaN stays one)
+  // a warp a row: its maximum and sum over the warps, and their weights (a sum of NaN stays one)
   for (int r = warp; r < rows; r += nw) {
     float mw = -INFINITY, lw = 0.f, mx;
     if (lane < nw) {
@@ -381,18 +361,12 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
       lw = part[lane * kPart + r * PITCH + HD + 1];
     }
     mx = mw;
-    for (int x = lane; x < n_parts; x += 32) mx = fmaxf(mx, part_m[r * kMaxParts + x]);
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int o = kRowsWarps / 2; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float ww = lw == 0.f ? 0.f : ex2(mw - mx);
     float sum = ww * lw;
-    for (int x = lane; x < n_parts; x += 32) {
-      const float l = part_w[r * kMaxParts + x], wt = l == 0.f ? 0.f : ex2(part_m[r * kMaxParts + x] - mx);
-      sum = fmaf(wt, l, sum);
-      part_w[r * kMaxParts + x] = wt;
-    }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = kRowsWarps / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane < nw) part[lane * kPart + r * PITCH + HD + 1] = ww;
     if (lane == 0) {
       total_of[2 * r] = mx;
@@ -402,8 +376,14 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
   if (nsplit > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   __syncthreads();
   const int Hq = p.Hkv * p.G;
-  auto put4 = [&](int r, int e, float4 v, float sum) {  // elements e .. e + 3 of the tile's row r
+  auto put4 = [&](int r, int e, float4 v, float mx, float sum) {  // elements e .. e + 3 of the tile's row r
     const int rr = row0 + r;
+    if (p.parts) {
+      float* to = p.parts + ((size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + rr / kTcRows) * p.n_parts + p.n_parts - 1) * part_floats(HD);
+      *reinterpret_cast<float4*>(to + (rr % kTcRows) * HD + e) = v;
+      if (e == 0) *reinterpret_cast<float2*>(to + kTcRows * HD + (rr % kTcRows) * 2) = make_float2(mx, sum);
+      return;
+    }
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.R + rr / p.G) * Hq + h * p.G + rr % p.G) * HD + e) =
         make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
@@ -418,16 +398,15 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
     };
 #pragma unroll 4
     for (int w = 0; w < nw; ++w) add(part[w * kPart + r * PITCH + HD + 1], *reinterpret_cast<const float4*>(part + w * kPart + r * PITCH + e));
-#pragma unroll 8
-    for (int x = 0; x < n_parts; ++x)
-      add(part_w[r * kMaxParts + x], *reinterpret_cast<const float4*>(from + size_t(x) * nsplit * part_floats(HD) + (row0 % kTcRows + r) * HD + e));
     if (nsplit == 1) {
-      put4(r, e, acc, total_of[2 * r + 1]);
+      put4(r, e, acc, total_of[2 * r], total_of[2 * r + 1]);
     } else {
       const uint32_t to = tc::mapa(tc::smem_u32(gathered + (rank * (ROWS * Q4 / nsplit) + i / nsplit) * 4), uint32_t(i) % nsplit);
       asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(acc.x), "f"(acc.y), "f"(acc.z), "f"(acc.w) : "memory");
     }
   }
+  // (who waits for this kernel waits for the one before it too)
+  if (p.parts) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nsplit == 1) return;
   for (int i = threadIdx.x; i < rows * int(nsplit); i += blockDim.x) {
     const int r = i / int(nsplit);
@@ -449,28 +428,28 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
       sum = fmaf(w, ml.y, sum);
       acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
     }
-    put4(r, e, acc, sum);
+    put4(r, e, acc, mx, sum);
   }
 }
 
 template <int HD, int MT>
-size_t rows_smem(int warps, bool parts) {
+size_t rows_smem(int warps) {
   constexpr int ROWS = 16 * MT;
-  return size_t(warps) * kStages * kChunkBytes + (ROWS * HD + 2 * kMaxSplit * ROWS + 2 * ROWS + (parts ? size_t(2) * ROWS * kMaxParts : 0)) * 4;
+  return size_t(warps) * kStages * kChunkBytes + (ROWS * HD + 2 * kMaxSplit * ROWS + 2 * ROWS) * 4;
 }
 
 // Blocks of `warps` warps, in clusters of `split`, that the device holds at once
 template <int HD, int MT, bool BF16>
-int64_t resident_blocks(int split, int warps, bool parts, int sm_count) {
-  static std::atomic<int> known[2][kMaxSplit + 1][kRowsWarps + 1];  // one kind of device: asked once per process
-  std::atomic<int>& k = known[parts][split][warps];
+int64_t resident_blocks(int split, int warps, int sm_count) {
+  static std::atomic<int> known[kMaxSplit + 1][kRowsWarps + 1];  // one kind of device: asked once per process
+  std::atomic<int>& k = known[split][warps];
   int n = k.load(std::memory_order_relaxed);
   if (n) return n;
   auto kern = rows_attn_kernel<HD, MT, BF16>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(split));
   cfg.blockDim = dim3(32 * warps);
-  cfg.dynamicSmemBytes = rows_smem<HD, MT>(warps, parts);
+  cfg.dynamicSmemBytes = rows_smem<HD, MT>(warps);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = split;
@@ -493,14 +472,14 @@ struct RowsChoice {
 // more in a cluster).  us by (warps, blocks): 1x5 rows on 1500 keys (6, 8) 5.5, (8, 4) 5.7, (4, 4) 6.0, (8, 8) 9.2 in two waves; 16x5 on 150..1500
 // (4, 1) 18.1, (6, 1) 17.5, (8, 1) 20.3, (4, 2) 20.6; 64x5 on 258 + 65 (6, 1) 34.4, (2, 1) 38.1, (4, 1) 42.3; 32x5 on 1500 (2, 1) 41.8, (4, 1) 44.9.
 template <int HD, int MT, bool BF16>
-RowsChoice choose_rows(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys, int64_t keys2, bool parts, int sm_count) {
+RowsChoice choose_rows(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys, int64_t keys2, int sm_count) {
   constexpr int ROWS = 16 * MT, KC = HD == 64 ? 32 : 16;
   const int64_t items = B * n_kv_heads * ((R * G + ROWS - 1) / ROWS);
   const int64_t chunks = (keys + KC - 1) / KC + std::min<int64_t>((ROWS - 1) / G + 1, R) * ((keys2 + KC - 1) / KC);
   RowsChoice best = {1, kRowsWarps, INT64_MAX};
   for (int s = 1; s <= kMaxSplit; s *= 2)
     for (int w = kRowsWarps; w >= 1; --w) {
-      const int64_t slots = resident_blocks<HD, MT, BF16>(s, w, parts, sm_count);
+      const int64_t slots = resident_blocks<HD, MT, BF16>(s, w, sm_count);
       const int64_t cost = (items * s + slots - 1) / slots * ((chunks + s * w - 1) / (s * w) + (s > 1 ? 4 : 3));
       if (cost < best.cost) best = {s, w, cost};
     }
@@ -510,7 +489,7 @@ RowsChoice choose_rows(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys
 template <int HD, int MT, bool BF16>
 int allow_rows() {  // what the occupancy query and the launch need set
   auto kern = rows_attn_kernel<HD, MT, BF16>;
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), rows_smem<HD, MT>(kRowsWarps, true));
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), rows_smem<HD, MT>(kRowsWarps));
   if (rc) return rc;
   ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return ASRQ_OK;
@@ -524,9 +503,9 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
   auto kern = rows_attn_kernel<HD, MT, BF16>;
   const int rc = allow_rows<HD, MT, BF16>();
   if (rc) return rc;
-  const RowsChoice choice = choose_rows<HD, MT, BF16>(B, p.R, p.G, p.Hkv, p.keys, p.k2 ? p.keys2 : 0, p.parts != nullptr, sm_count);
+  const RowsChoice choice = choose_rows<HD, MT, BF16>(B, p.R, p.G, p.Hkv, p.keys, p.k2 ? p.keys2 : 0, sm_count);
   const int split = choice.split, warps = choice.warps;
-  const size_t smem = rows_smem<HD, MT>(warps, p.parts != nullptr);
+  const size_t smem = rows_smem<HD, MT>(warps);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(items * split));
   cfg.blockDim = dim3(32 * warps);
@@ -547,10 +526,10 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
 }  // namespace
 
 // The row kernel's time in us, by its units above: 1.2 each, more with many dimensions or rows to a warp (measured: 1.1 to 1.5, 1.2 to 1.5, 1.6 to 1.75).
-double rows_estimate(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, int64_t keys2, bool parts, int sm_count) {
-  if (hd == 128) return 1.3 * double(choose_rows<128, 1, false>(B, R, G, n_kv_heads, keys, keys2, parts, sm_count).cost);
-  if (R * G > 16) return 1.65 * double(choose_rows<64, 2, false>(B, R, G, n_kv_heads, keys, keys2, parts, sm_count).cost);
-  return 1.2 * double(choose_rows<64, 1, false>(B, R, G, n_kv_heads, keys, keys2, parts, sm_count).cost);
+double rows_estimate(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
+  if (hd == 128) return 1.3 * double(choose_rows<128, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
+  if (R * G > 16) return 1.65 * double(choose_rows<64, 2, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
+  return 1.2 * double(choose_rows<64, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
 }
 
 // Whether the tensor-core kernel takes a call, and how it divides it.  It walks tiles of keys at 1.3 us a wave of blocks, with 3 for a block's start
@@ -575,8 +554,8 @@ TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys
   }
   if (forced == 2) return plan;
   double us = 1.3 * double(first + least);
-  if (own) us += rows_estimate(B, R, G, n_kv_heads, hd, 0, keys2, true, sm_count);
-  return us < rows_estimate(B, R, G, n_kv_heads, hd, keys, keys2, false, sm_count) ? plan : TcPlan{0, 0};
+  if (own) us += rows_estimate(B, R, G, n_kv_heads, hd, 0, keys2, sm_count);
+  return us < rows_estimate(B, R, G, n_kv_heads, hd, keys, keys2, sm_count) ? plan : TcPlan{0, 0};
 }
 int allow_all() {
   int rc = allow_rows<64, 1, false>();
@@ -584,14 +563,15 @@ int allow_all() {
   if (!rc) rc = allow_rows<128, 1, false>();
   return rc;
 }
-size_t part_bytes(int64_t B, int64_t R, int G, int n_kv_heads, int hd, const TcPlan& plan) {
+size_t part_bytes(int64_t B, int64_t R, int G, int n_kv_heads, int hd, const TcPlan& plan, bool own) {
+  if (plan.split == 0) return 0;
   const int64_t items = B * n_kv_heads * ((R * G + kTcRows - 1) / kTcRows);
-  return size_t(items - plan.whole) * plan.split * part_floats(hd) * sizeof(float);
+  return size_t(items - plan.whole) * (plan.split + own) * part_floats(hd) * sizeof(float);
 }
 
 size_t rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
   const int G = n_q_heads / n_kv_heads;
-  return allow_all() ? 0 : part_bytes(B, R, G, n_kv_heads, hd, tc_plan(B, R, G, n_kv_heads, hd, keys, keys2, sm_count));
+  return allow_all() ? 0 : part_bytes(B, R, G, n_kv_heads, hd, tc_plan(B, R, G, n_kv_heads, hd, keys, keys2, sm_count), keys2 > 0);
 }
 
 int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
@@ -617,25 +597,33 @@ int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_
   p.scale_log2 = scale * 1.4426950408889634f;
   const bool bf16 = dtype == ASRQ_BF16;
   TcPlan plan = {0, 0};
+  auto launch = [&](const RowsParams& x) {
+    if (hd == 128) return bf16 ? launch_rows<128, 1, true>(x, B, sm_count, stream) : launch_rows<128, 1, false>(x, B, sm_count, stream);
+    if (R * x.G > 16) return bf16 ? launch_rows<64, 2, true>(x, B, sm_count, stream) : launch_rows<64, 2, false>(x, B, sm_count, stream);
+    return bf16 ? launch_rows<64, 1, true>(x, B, sm_count, stream) : launch_rows<64, 1, false>(x, B, sm_count, stream);
+  };
   int rc = allow_all();
   if (rc) return rc;
   // (the tensor-core kernel copies keys at a stride, and hides scores before it scales them)
   if (status && ((ks[2] && vs[2]) || keys == 1) && p.scale_log2 != 0.f) plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
   if (plan.split > 0) {
-    const size_t need = part_bytes(B, R, p.G, n_kv_heads, hd, plan);
+    const size_t need = part_bytes(B, R, p.G, n_kv_heads, hd, plan, k2 != nullptr);
     const bool kept = need == 0 || (scratch && scratch_bytes >= need);
     if (!kept && !k2) plan = {B * n_kv_heads * ((R * p.G + kTcRows - 1) / kTcRows), 1};
     if (kept || !k2) {
-      rc = rows_attention_tc(p, hd, bf16, B, plan, need && kept ? static_cast<float*>(scratch) : nullptr, !k2, status, stream);
-      if (rc || !k2) return rc;
-      p.parts = static_cast<const float*>(scratch);
-      p.n_parts = plan.split;
-      p.keys = 0;
+      float* parts = need && kept ? static_cast<float*>(scratch) : nullptr;
+      rc = rows_attention_tc(p, hd, bf16, B, plan, parts, k2 ? 1 : 0, status, stream);
+      if (!rc && k2) {
+        RowsParams own = p;
+        own.keys = 0;
+        own.parts = parts;
+        own.n_parts = plan.split + 1;
+        rc = launch(own);
+      }
+      return rc ? rc : rows_attention_join(p, hd, bf16, B, plan.whole, parts, plan.split + (k2 ? 1 : 0), stream);
     }
   }
-  if (hd == 128) return bf16 ? launch_rows<128, 1, true>(p, B, sm_count, stream) : launch_rows<128, 1, false>(p, B, sm_count, stream);
-  if (R * p.G > 16) return bf16 ? launch_rows<64, 2, true>(p, B, sm_count, stream) : launch_rows<64, 2, false>(p, B, sm_count, stream);
-  return bf16 ? launch_rows<64, 1, true>(p, B, sm_count, stream) : launch_rows<64, 1, false>(p, B, sm_count, stream);
+  return launch(p);
 }
 
 }  // namespace asrq

@@ -15,12 +15,12 @@ struct RowsParams {
   long long keys, keys2;         // room
   int len2_many, R, G, Hkv, tiles;
   float scale_log2;              // scale * log2 e
-  // What the tensor-core kernel leaves of the shared keys, for a row kernel to join: for every utterance, key head, tile of 128 rows and part
-  // 128 x HD values, then 128 pairs of maximum (as an exponent of two) and sum.
-  const float* parts;
+  // Where the shared keys are the tensor-core kernel's, a row kernel leaves its rows' own keys as one more part: for every utterance, key head and tile of
+  // 128 rows n_parts parts, each 128 x HD values, then 128 pairs of maximum (as an exponent of two) and sum.  The row kernel's is the last.
+  float* parts;
   int n_parts;
 };
-constexpr int kTcRows = 128;
+constexpr int kTcRows = 128, kMaxParts = 64;  // rows of its tile; parts it divides an item's keys into at most
 __host__ __device__ constexpr int part_floats(int hd) { return kTcRows * (hd + 2); }
 
 // How the tensor-core kernel divides a call's items (utterance, key head, 128 rows): the first `whole` have a block each, the keys of the others
@@ -30,7 +30,10 @@ struct TcPlan {
   int split;
 };
 
-// The shared keys of p by tcgen05.  join: the parts are joined to results; else they are left for a row kernel (whole is 0 then).
-int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, bool join, void* status, cudaStream_t stream);
+// The shared keys of p by tcgen05; room is left behind every item's parts for `more` of them.
+int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, cudaStream_t stream);
+
+// The results of the items from `whole` on, from n_parts parts each.
+int rows_attention_join(const RowsParams& p, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, int n_parts, cudaStream_t stream);
 
 }  // namespace asrq

@@ -26,7 +26,8 @@ struct FlashParams {
   float* parts;
   unsigned* status;
   long long q_b, q_r, q_h, keys;
-  int R, G, Hkv, tiles, whole, split, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
+  int R, G, Hkv, tiles, whole, split, slots, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
+  // slots: parts of an item, `split` of them this kernel's
   float scale_log2;  // not negative
   uint32_t q_flip;   // the sign bits of a query pair where the scale is
 };
@@ -366,7 +367,7 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     tc::fence_after_sync();
     if (m == -INFINITY && sum == sum) sum = 0.f;  // nothing above -inf
     const int rr = row0 + r;
-    float* to = p.parts && !alone ? p.parts + size_t(rest) * part_floats(HD) : nullptr;
+    float* to = p.parts && !alone ? p.parts + (size_t(rest / split) * p.slots + part) * part_floats(HD) : nullptr;
     uint16_t* out = p.out + ((size_t(b) * p.R + rr / p.G) * (p.Hkv * p.G) + h * p.G + rr % p.G) * HD;
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
@@ -398,31 +399,71 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
   if (warp == 1) tc::tmem_dealloc(tmem, 256);
 }
 
-// The results of items that several blocks share: a thread for 4 dimensions of a row, 128 a block.
-constexpr int kJoinThreads = 128;
-template <int HD, bool BF16>
+// The results of items that several blocks share: WARPS warps a row, 256 / (32 WARPS) rows a block.  The row's warps (half warps with 64 dimensions)
+// take its parts in turn, all loads at once.  Two warps a row up to 16 parts (3072 rows of 10 parts, us: two 3.1, eight 9.0), else eight.
+constexpr int kJoinThreads = 256;
+template <int HD, bool BF16, int WARPS>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float* parts, uint16_t* out, int n_parts, int first_item, int tiles, int R, int G, int Hkv) {
-  constexpr int PER = HD / 4, ROWS = kJoinThreads / PER, BLOCKS = kTcRows / ROWS;  // threads of a row, rows of a block, blocks of an item
+  constexpr int PER = HD / 4, TEAMS = 32 * WARPS / PER, ROWS = kJoinThreads / (32 * WARPS);  // threads of a part, parts at a time, rows
+  constexpr int kMost = WARPS == 2 ? 16 : kMaxParts + 1;
+  __shared__ float4 sums[ROWS][TEAMS][PER];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int at = int(blockIdx.x) / BLOCKS, item = first_item + at, bh = item / tiles, h = bh % Hkv, b = bh / Hkv;
-  const int r = (int(blockIdx.x) % BLOCKS) * ROWS + int(threadIdx.x) / PER, rr = (item % tiles) * kTcRows + r, e = (int(threadIdx.x) % PER) * 4;
-  if (rr >= R * G) return;
+  const int in_block = int(threadIdx.x) / (32 * WARPS), thread = int(threadIdx.x) % (32 * WARPS);
+  const int at = int(blockIdx.x) / (kTcRows / ROWS), r = int(blockIdx.x) % (kTcRows / ROWS) * ROWS + in_block, item = first_item + at;
+  const int rr = (item % tiles) * kTcRows + r;
+  const bool there = rr < R * G;  // (else it reads what nobody wrote, and writes nothing)
+  const int lane = threadIdx.x & 31, team = thread / PER, e = (thread % PER) * 4;
   const float* from = behind_wait(parts + size_t(at) * n_parts * part_floats(HD));
+  const float *ml = from + kTcRows * HD + r * 2, *row = from + r * HD + e;
+  constexpr int kEach = (kMost + TEAMS - 1) / TEAMS, kLists = (kMost + 31) / 32;
+  float4 o[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int x = i * TEAMS + team;
+    o[i] = x < n_parts ? *reinterpret_cast<const float4*>(row + size_t(x) * part_floats(HD)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // every warp: maxima and sums of all parts, two or three a lane
+  float2 own[kLists];
   float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kLists; ++i) {
+    const int x = i * 32 + lane;
+    own[i] = x < n_parts ? *reinterpret_cast<const float2*>(ml + size_t(x) * part_floats(HD)) : make_float2(-INFINITY, 0.f);
+    mx = fmaxf(mx, own[i].x);
+  }
+#pragma unroll
+  for (int s = 16; s >= 1; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+#pragma unroll
+  for (int i = 0; i < kLists; ++i) {
+    const float w = own[i].y == 0.f ? 0.f : ex2f(own[i].x - mx);  // (a sum of NaN stays one)
+    sum = fmaf(w, own[i].y, sum);
+    own[i].x = w;
+  }
+#pragma unroll
+  for (int s = 16; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int x = 0; x < n_parts; ++x) mx = fmaxf(mx, from[size_t(x) * part_floats(HD) + kTcRows * HD + r * 2]);
-#pragma unroll 8
-  for (int x = 0; x < n_parts; ++x) {
-    const float* d = from + size_t(x) * part_floats(HD);
-    const float2 ml = *reinterpret_cast<const float2*>(d + kTcRows * HD + r * 2);
-    const float4 o = *reinterpret_cast<const float4*>(d + r * HD + e);
-    const float w = ml.y == 0.f ? 0.f : ex2f(ml.x - mx);  // (a sum of NaN stays one)
-    sum = fmaf(w, ml.y, sum);
-    acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int x = i * TEAMS + team;  // its weight: with lane x % 32
+    float w = 0.f;
+#pragma unroll
+    for (int j = 0; j < kLists; ++j) {
+      const float v = __shfl_sync(0xffffffffu, own[j].x, x & 31);
+      if (x / 32 == j) w = v;
+    }
+    if (x < n_parts) acc.x = fmaf(w, o[i].x, acc.x), acc.y = fmaf(w, o[i].y, acc.y), acc.z = fmaf(w, o[i].z, acc.z), acc.w = fmaf(w, o[i].w, acc.w);
+  }
+  sums[in_block][team][e / 4] = acc;
+  __syncthreads();
+  if (team != 0 || !there) return;
+#pragma unroll
+  for (int i = 1; i < TEAMS; ++i) {
+    const float4 v = sums[in_block][i][e / 4];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
   }
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const int bh = item / tiles, h = bh % Hkv, b = bh / Hkv;
   *reinterpret_cast<uint2*>(out + ((size_t(b) * R + rr / G) * (Hkv * G) + h * G + rr % G) * HD + e) =
       make_uint2(pack16<BF16>(acc.x * inv, acc.y * inv), pack16<BF16>(acc.z * inv, acc.w * inv));
 }
@@ -444,18 +485,30 @@ int launch_behind(void (*kern)(Args...), int64_t blocks, int threads, size_t sme
 }
 
 template <int HD, bool BF16>
-int launch_flash(const CUtensorMap& kmap, const CUtensorMap& vmap, const FlashParams& p, int64_t items, bool join, cudaStream_t stream) {
+int launch_flash(const CUtensorMap& kmap, const CUtensorMap& vmap, const FlashParams& p, int64_t items, cudaStream_t stream) {
   auto kern = flash_kernel<HD, BF16>;
-  int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FlashLayout<HD>::kBytes);
-  if (!rc) rc = launch_behind(kern, p.whole + (items - p.whole) * p.split, 192, FlashLayout<HD>::kBytes, stream, kmap, vmap, p);
-  if (!rc && join && p.whole < items)
-    rc = launch_behind(join_kernel<HD, BF16>, (items - p.whole) * (kTcRows * HD / 4 / kJoinThreads), kJoinThreads, 0, stream, (const float*)p.parts, p.out, p.split, p.whole, p.tiles, p.R, p.G, p.Hkv);
-  return rc;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FlashLayout<HD>::kBytes);
+  return rc ? rc : launch_behind(kern, p.whole + (items - p.whole) * p.split, 192, FlashLayout<HD>::kBytes, stream, kmap, vmap, p);
 }
 
 }  // namespace
 
-int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, bool join, void* status, cudaStream_t stream) {
+int rows_attention_join(const RowsParams& r, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, int n_parts, cudaStream_t stream) {
+  const int tiles = (r.R * r.G + kTcRows - 1) / kTcRows;
+  const int64_t items = B * r.Hkv * tiles;
+  if (whole >= items) return ASRQ_OK;
+  auto go = [&](auto kern, int rows) {
+    return launch_behind(kern, (items - whole) * (kTcRows / rows), kJoinThreads, 0, stream, parts, r.out, n_parts, int(whole), tiles, r.R, r.G, r.Hkv);
+  };
+  if (n_parts <= 16) {
+    if (hd == 64) return bf16 ? go(join_kernel<64, true, 2>, 4) : go(join_kernel<64, false, 2>, 4);
+    return bf16 ? go(join_kernel<128, true, 2>, 4) : go(join_kernel<128, false, 2>, 4);
+  }
+  if (hd == 64) return bf16 ? go(join_kernel<64, true, 8>, 1) : go(join_kernel<64, false, 8>, 1);
+  return bf16 ? go(join_kernel<128, true, 8>, 1) : go(join_kernel<128, false, 8>, 1);
+}
+
+int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, cudaStream_t stream) {
   FlashParams p = {};
   p.q = r.q, p.out = r.out, p.len = r.len;
   p.parts = parts;
@@ -465,6 +518,7 @@ int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const T
   p.tiles = (r.R * r.G + kTcRows - 1) / kTcRows;
   p.whole = int(plan.whole);
   p.split = plan.split;
+  p.slots = plan.split + more;
   p.scale_log2 = r.scale_log2 < 0.f ? -r.scale_log2 : r.scale_log2;
   p.q_flip = r.scale_log2 < 0.f ? 0x80008000u : 0u;
   p.k_batch = r.k_b != 0, p.v_batch = r.v_b != 0, p.k_head = r.k_h != 0, p.v_head = r.v_h != 0;
@@ -474,8 +528,8 @@ int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const T
   if (!rc) rc = make_tmap_4d(&vmap, r.v, bf16, hd, uint64_t(r.keys), r.v_h ? r.Hkv : 1, r.v_b ? uint64_t(B) : 1, r.v_t, r.v_h, r.v_b, 64, keys);
   if (rc) return rc;
   const int64_t items = B * p.Hkv * p.tiles;
-  if (hd == 64) return bf16 ? launch_flash<64, true>(kmap, vmap, p, items, join, stream) : launch_flash<64, false>(kmap, vmap, p, items, join, stream);
-  return bf16 ? launch_flash<128, true>(kmap, vmap, p, items, join, stream) : launch_flash<128, false>(kmap, vmap, p, items, join, stream);
+  if (hd == 64) return bf16 ? launch_flash<64, true>(kmap, vmap, p, items, stream) : launch_flash<64, false>(kmap, vmap, p, items, stream);
+  return bf16 ? launch_flash<128, true>(kmap, vmap, p, items, stream) : launch_flash<128, false>(kmap, vmap, p, items, stream);
 }
 
 }  // namespace asrq
