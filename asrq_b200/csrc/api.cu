@@ -257,14 +257,17 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, bool bf16, 
   return ASRQ_OK;
 }
 
-int make_tmap_4d(CUtensorMap* out, const void* base, bool bf16, uint64_t inner, uint64_t d1, uint64_t d2, uint64_t d3, int64_t s1, int64_t s2, int64_t s3,
-                 uint32_t box_inner, uint32_t box_1) {
+int make_tmap_rows(CUtensorMap* out, const void* base, bool bf16, uint64_t inner, uint32_t box_inner, const TmapDim* d, int n) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(ASRQ_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
-  auto bytes = [&](uint64_t d, int64_t s) { return d > 1 ? cuuint64_t(s) * 2 : cuuint64_t(inner) * 2; };
-  const cuuint64_t dims[4] = {inner, d1, d2, d3}, strides[3] = {bytes(d1, s1), bytes(d2, s2), bytes(d3, s3)};
-  const cuuint32_t box[4] = {box_inner, box_1, 1, 1}, estr[4] = {1, 1, 1, 1};
-  const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+  cuuint64_t dims[5] = {inner}, strides[4];
+  cuuint32_t box[5] = {box_inner}, estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < n; ++i) {
+    dims[i + 1] = d[i].size;
+    strides[i] = d[i].size > 1 ? cuuint64_t(d[i].stride) * 2 : cuuint64_t(inner) * 2;
+    box[i + 1] = d[i].box;
+  }
+  const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, cuuint32_t(n + 1), const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(ASRQ_ERR_SHAPE, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
   return ASRQ_OK;

@@ -541,7 +541,7 @@ TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys
   const int64_t key_tiles = (keys + step - 1) / step, slots = 2 * sm_count;
   const bool own = keys2 > 0;
   const int forced = option(kOptRowsKernel);
-  if (keys == 0 || forced == 1 || (forced != 2 && (rows <= 16 || keys < 64))) return {0, 0};
+  if (keys == 0 || kTcRows % G != 0 || forced == 1 || (forced != 2 && (rows <= 16 || keys < 64))) return {0, 0};
   const int64_t whole = own ? 0 : items / slots * slots, rest = items - whole, first = whole / slots * (key_tiles + 3);
   TcPlan plan = {own ? 0 : items, own ? 0 : 1};
   int64_t least = rest == 0 ? 0 : own ? INT64_MAX : key_tiles + 3;
@@ -604,15 +604,17 @@ int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_
   };
   int rc = allow_all();
   if (rc) return rc;
-  // (the tensor-core kernel copies keys at a stride, and hides scores before it scales them)
-  if (status && ((ks[2] && vs[2]) || keys == 1) && p.scale_log2 != 0.f) plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
+  // (the tensor-core kernel's copies know no two elements at one place but along whole dimensions of keys, and it hides scores before it scales them)
+  auto apart = [](int64_t n, int64_t stride) { return n == 1 || stride != 0; };
+  if (status && p.scale_log2 > 0.f && apart(keys, ks[2]) && apart(keys, vs[2]) && apart(B, qs[0]) && apart(R, qs[1]) && apart(n_q_heads, qs[2]))
+    plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
   if (plan.split > 0) {
     const size_t need = part_bytes(B, R, p.G, n_kv_heads, hd, plan, k2 != nullptr);
     const bool kept = need == 0 || (scratch && scratch_bytes >= need);
     if (!kept && !k2) plan = {B * n_kv_heads * ((R * p.G + kTcRows - 1) / kTcRows), 1};
     if (kept || !k2) {
       float* parts = need && kept ? static_cast<float*>(scratch) : nullptr;
-      rc = rows_attention_tc(p, hd, bf16, B, plan, parts, k2 ? 1 : 0, status, stream);
+      rc = rows_attention_tc(p, hd, bf16, B, plan, parts, k2 ? 1 : 0, status, sm_count, stream);
       if (!rc && k2) {
         RowsParams own = p;
         own.keys = 0;

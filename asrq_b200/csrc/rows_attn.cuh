@@ -31,7 +31,8 @@ struct TcPlan {
 };
 
 // The shared keys of p by tcgen05; room is left behind every item's parts for `more` of them.
-int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, cudaStream_t stream);
+int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, int sm_count,
+                      cudaStream_t stream);
 
 // The results of the items from `whole` on, from n_parts parts each.
 int rows_attention_join(const RowsParams& p, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, int n_parts, cudaStream_t stream);

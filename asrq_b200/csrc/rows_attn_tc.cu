@@ -5,12 +5,15 @@
 // time: S = Q K^T into tensor memory, a thread per row reads its scores, and writes the weights 2^(scale' s - m) in 16 bits to tensor memory
 // too, from where O += P V takes them as its first operand.  K arrives by TMA as rows of the contraction, V as it lies, dimensions
 // contiguous, which the second operand's descriptor calls MN-major.  The next S is on its way as soon as the scores are in registers, and
-// two blocks an SM fill each other's waits.
+// two blocks an SM fill each other's waits.  Blocks stay and take one item after the other: the next one's queries and keys arrive and its first S is
+// done while the last weights and the result of the one before are.
 // The reference exponent m of a row moves only when its maximum has grown by more than 8 (a weight stays below 2^8, a sum in 32 bits has
 // room for that): O is scaled at the first tiles and hardly ever after.
 //
 // Bound: at 64 dimensions the exponentials, 16 a cycle and SM, of which every fourth pair goes to the multipliers instead; at 128 these and the
 // memory's bytes where few rows share many keys.
+#include <algorithm>
+
 #include "rows_attn.cuh"
 
 namespace asrq {
@@ -20,16 +23,14 @@ int ensure_dynamic_smem(const void* kernel, size_t bytes);
 namespace {
 
 struct FlashParams {
-  const uint16_t* q;
   uint16_t* out;
   const long long* len;
   float* parts;
   unsigned* status;
-  long long q_b, q_r, q_h, keys;
-  int R, G, Hkv, tiles, whole, split, slots, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
-  // slots: parts of an item, `split` of them this kernel's
-  float scale_log2;  // not negative
-  uint32_t q_flip;   // the sign bits of a query pair where the scale is
+  long long keys;
+  int R, G, Hkv, tiles, units, whole, split, slots, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
+  // units: what a block takes at a time; the first `whole` are items, the others parts of items, `split` of each; slots: parts of an item there is room for
+  float scale_log2;  // positive
 };
 
 template <int HD>
@@ -38,13 +39,19 @@ struct FlashLayout {
   static constexpr int kStages = HD == 64 ? 3 : 2;
   static constexpr int kQ = kTcRows * HD * 2, kTile = kKeys * HD * 2;
   static constexpr int kK = kQ, kV = kQ + kStages * kTile, kBars = kQ + 2 * kStages * kTile;
-  static constexpr int kBytes = kBars + (4 * kStages + 4) * 8 + 16 + 1024;  // 1024: the base is aligned to it
+  static constexpr int kBytes = kBars + (4 * kStages + 7) * 8 + 16 + 1024;  // 1024: the base is aligned to it
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, int c4, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
 // MN-major operand with 128-byte swizzle: 64 values along N contiguous, 8 k apart by 128 bytes each, groups of 8 k 1024 bytes apart; the
@@ -129,7 +136,7 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, unsigned* st
 
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(192, 2)
-flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FlashParams p) {
+flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FlashParams p) {
   using L = FlashLayout<HD>;
   constexpr int ST = L::kStages, HALVES = HD / 64, kKeys = L::kKeys;
   constexpr uint32_t kP = kKeys, kOut = 256 - HD;  // columns of tensor memory: the scores from 0, the weights, the result
@@ -143,102 +150,109 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
   auto k_free = [&](int s) { return bar(ST + s); };
   auto v_full = [&](int s) { return bar(2 * ST + s); };
   auto v_free = [&](int s) { return bar(3 * ST + s); };
-  const uint32_t s_full = bar(4 * ST), s_free = bar(4 * ST + 1), p_full = bar(4 * ST + 2), o_done = bar(4 * ST + 3);
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kBars + (4 * ST + 4) * 8);
+  const uint32_t s_full = bar(4 * ST), s_free = bar(4 * ST + 1), p_full = bar(4 * ST + 2), o_done = bar(4 * ST + 3), q_full = bar(4 * ST + 4), o_free = bar(4 * ST + 5), q_free = bar(4 * ST + 6);
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kBars + (4 * ST + 7) * 8);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4 * ST + 4; ++i) tc::mbar_init(bar(i), bar(i) == s_free || bar(i) == p_full ? 4 : 1);
+    for (int i = 0; i < 4 * ST + 7; ++i) {
+      const uint32_t x = bar(i);
+      tc::mbar_init(x, x == s_free || x == p_full || x == o_free ? 4 : 1);  // from each softmax warp
+    }
     tc::fence_barrier_init();
+    tc::prefetch_tmap(&qmap);
     tc::prefetch_tmap(&kmap);
     tc::prefetch_tmap(&vmap);
   }
-  // the first `whole` items by a block each, the others by `split`
-  const bool alone = int(blockIdx.x) < p.whole;
-  const int rest = int(blockIdx.x) - p.whole, split = alone ? 1 : p.split, part = alone ? 0 : rest % p.split;
-  const int item = alone ? int(blockIdx.x) : p.whole + rest / p.split;
-  const int tile = item % p.tiles, bh = item / p.tiles, h = bh % p.Hkv, b = bh / p.Hkv;
-  const int row0 = tile * kTcRows, rows = min(kTcRows, p.R * p.G - row0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  // Q on its way first: all warps but the one that starts the copies
-  constexpr int kChunks = kTcRows * HD / 8, kEach = (kChunks + 159) / 160;
-  uint4 u[kEach];
-  const uint16_t* q = p.q + b * p.q_b + (long long)(h * p.G) * p.q_h;
-  const int q0 = int(threadIdx.x) - 32;
-#pragma unroll
-  for (int x = 0; x < kEach; ++x) {
-    const int i = x * 160 + q0, r = i / (HD / 8), c = i % (HD / 8), rr = row0 + r;
-    const int token = p.G == 1 ? rr : rr / p.G;
-    u[x] = make_uint4(0, 0, 0, 0);
-    if (q0 >= 0 && r < rows) u[x] = ld_x4(q + token * p.q_r + (long long)(rr - token * p.G) * p.q_h + c * 8);
-  }
-  const long long n_keys = p.len ? min(max(*(const volatile long long*)(p.len + b), 0ll), p.keys) : p.keys;
-  // (fewer than 2^25 tiles, at most 64 parts)
-  const int all = int((n_keys + kKeys - 1) / kKeys), t0 = int(unsigned(all) * unsigned(part) / unsigned(split));
-  const int n = int(unsigned(all) * unsigned(part + 1) / unsigned(split)) - t0;
-  // Tensor memory only behind the wait, and the next kernel only behind it: a block that held it while it waits could keep it from one that it
-  // waits for.
-  if (warp == 1) {
-    tc::tmem_alloc(tc::smem_u32(tmem_at), 256);
-    tc::tmem_relinquish();
-  }
-  const int last_keys = t0 + n == all ? int(n_keys - (long long)(all - 1) * kKeys) : kKeys;  // of this block's last tile
-
-  const int kb = p.k_batch ? b : 0, kh = p.k_head ? h : 0, vb = p.v_batch ? b : 0, vh = p.v_head ? h : 0;
-  auto load_k = [&](int j) {
-    const int s = j % ST;
-    tc::mbar_arrive_expect_tx(k_full(s), L::kTile);
-    for (int x = 0; x < HALVES; ++x) tma_load_4d(base + L::kK + uint32_t(s * L::kTile + x * kKeys * 128), &kmap, x * 64, (t0 + j) * kKeys, kh, kb, k_full(s));
-  };
-  auto load_v = [&](int j) {
-    const int s = j % ST;
-    tc::mbar_arrive_expect_tx(v_full(s), L::kTile);
-    for (int x = 0; x < HALVES; ++x) tma_load_4d(base + L::kV + uint32_t(s * L::kTile + x * kKeys * 128), &vmap, x * 64, (t0 + j) * kKeys, vh, vb, v_full(s));
-  };
-  if (threadIdx.x == 0)  // the thread that made the barriers
-    for (int j = 0; j < min(n, ST); ++j) {
-      load_k(j);
-      load_v(j);
-    }
-  // Q, rows of the contraction, 64 dimensions (128 bytes, chunks of 16 exchanged by the row) at a time
-#pragma unroll
-  for (int x = 0; x < kEach; ++x) {
-    const int i = x * 160 + q0, r = i / (HD / 8), c = i % (HD / 8);
-    if (q0 >= 0 && i < kChunks)
-      tc::st_shared_v4(base + uint32_t((c / 8) * kTcRows * 128 + r * 128 + (((c % 8) ^ (r & 7)) * 16)), u[x].x ^ p.q_flip, u[x].y ^ p.q_flip, u[x].z ^ p.q_flip,
-                       u[x].w ^ p.q_flip);
-  }
-  tc::fence_proxy_async_smem();
-  tc::fence_before_sync();
   __syncthreads();
-  tc::fence_after_sync();
-  const uint32_t tmem = *(volatile uint32_t*)tmem_at;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  if (warp == 0) {
-    if (lane == 0 && n > 0) {
+  struct Unit {
+    int b, h, row0, rows, rest;     // rest: which part in memory, negative: the result itself
+    int t0, n, last_keys;           // its tiles of keys, and the keys of the last one
+  };
+  auto unit = [&](int u) {
+    Unit w;
+    const bool alone = u < p.whole;
+    const int rest = u - p.whole, split = alone ? 1 : p.split, at = alone ? 0 : rest / split, part = alone ? 0 : rest - at * split;
+    const int item = alone ? u : p.whole + at, bh = item / p.tiles;
+    w.rest = alone || !p.parts ? -1 : at * p.slots + part;
+    w.b = bh / p.Hkv;
+    w.h = bh - w.b * p.Hkv;
+    w.row0 = (item - bh * p.tiles) * kTcRows;
+    w.rows = min(kTcRows, p.R * p.G - w.row0);
+    const long long n_keys = p.len ? min(max(*(const volatile long long*)(p.len + w.b), 0ll), p.keys) : p.keys;
+    // (fewer than 2^25 tiles, at most 64 parts)
+    const unsigned all = unsigned((n_keys + kKeys - 1) / kKeys);
+    w.t0 = int(all * unsigned(part) / unsigned(split));
+    w.n = int(all * unsigned(part + 1) / unsigned(split)) - w.t0;
+    w.last_keys = w.t0 + w.n == int(all) ? int(n_keys - (long long)(int(all) - 1) * kKeys) : kKeys;
+    return w;
+  };
+  const int step = int(gridDim.x);
+
+  if (warp == 0) {  // the copies, tile by tile through all units
+    if (lane == 0) {
       bool ok = true;
-      for (int j = ST; j < n && ok; ++j) {
-        const int s = j % ST;
-        const uint32_t ph = uint32_t(j / ST) & 1u;
-        ok = wait(k_free(s), ph ^ 1u, p.status, 61);
-        if (!ok) break;
-        load_k(j);
-        ok = wait(v_free(s), ph ^ 1u, p.status, 62);
-        if (ok) load_v(j);
-      }
-      if (!ok)  // copies that are on their way still land here
-        for (int s = 0; s < ST; ++s) {
-          wait(k_full(s), 0, p.status, 63);
-          wait(v_full(s), 0, p.status, 63);
+      int t = 0, v_started = 0, taken = 0;
+      for (int x = int(blockIdx.x); x < p.units && ok; x += step) {
+        const Unit w = unit(x);
+        const int kb = p.k_batch ? w.b : 0, kh = p.k_head ? w.h : 0, vb = p.v_batch ? w.b : 0, vh = p.v_head ? w.h : 0;
+        for (int j = 0; j < w.n; ++j, ++t) {
+          const int s = t % ST, at = (w.t0 + j) * kKeys;
+          const uint32_t ph = (uint32_t(t / ST) & 1u) ^ 1u;
+          ok = wait(k_free(s), ph, p.status, 61);
+          if (!ok) break;
+          tc::mbar_arrive_expect_tx(k_full(s), L::kTile);
+          for (int i = 0; i < HALVES; ++i) tma_load_4d(base + L::kK + uint32_t(s * L::kTile + i * kKeys * 128), &kmap, i * 64, at, kh, kb, k_full(s));
+          ok = wait(v_free(s), ph, p.status, 62);
+          if (!ok) {
+            ++t;
+            break;
+          }
+          tc::mbar_arrive_expect_tx(v_full(s), L::kTile);
+          for (int i = 0; i < HALVES; ++i) tma_load_4d(base + L::kV + uint32_t(s * L::kTile + i * kKeys * 128), &vmap, i * 64, at, vh, vb, v_full(s));
+          ++v_started;
+          if (j == 0) {  // the queries' place: free when the last scores of the unit before are done
+            if (taken > 0) ok = wait(q_free, uint32_t(taken - 1) & 1u, p.status, 73);
+            if (!ok) {
+              ++t;
+              break;
+            }
+            tc::mbar_arrive_expect_tx(q_full, L::kQ);
+            for (int i = 0; i < HALVES; ++i) tma_load_5d(base + uint32_t(i * kTcRows * 128), &qmap, i * 64, 0, w.row0 / p.G, w.h, w.b, q_full);
+            ++taken;
+          }
         }
+      }
+      if (!ok) {  // copies that are on their way still land here
+        for (int i = max(t - ST, 0); i < t; ++i) wait(k_full(i % ST), uint32_t(i / ST) & 1u, p.status, 63);
+        for (int i = max(v_started - ST, 0); i < v_started; ++i) wait(v_full(i % ST), uint32_t(i / ST) & 1u, p.status, 63);
+        if (taken > 0) wait(q_full, uint32_t(taken - 1) & 1u, p.status, 63);
+      }
     }
-  } else if (warp == 1) {
+  } else {
+    // Tensor memory only behind the wait, and the next kernel only behind it: a block that held it while it waits could keep it from one that it
+    // waits for.
+    if (warp == 1) {
+      tc::tmem_alloc(tc::smem_u32(tmem_at), 256);
+      tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    asm volatile("bar.sync 1, 160;" ::: "memory");
+    tc::fence_after_sync();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  }
+  const uint32_t tmem = warp == 0 ? 0u : *(volatile uint32_t*)tmem_at;
+
+  if (warp == 1) {
     const uint32_t s_desc = tc::instr_desc(1, BF16 ? 1 : 0, kTcRows, kKeys), o_desc = tc::instr_desc(1, BF16 ? 1 : 0, kTcRows, HD) | (1u << 16);
     const bool one = tc::elect_one();
     bool ok = true;
-    auto scores = [&](int j) {  // of tile j
-      const int s = j % ST;
-      if (!__all_sync(0xffffffffu, wait(k_full(s), uint32_t(j / ST) & 1u, p.status, 64))) return false;
+    auto all_wait = [&](uint32_t b, uint32_t parity, unsigned site) { return bool(__all_sync(0xffffffffu, wait(b, parity, p.status, site))); };
+    auto scores = [&](int t, bool last) {  // of the block's tile t, the last of its unit
+      const int s = t % ST;
+      if (!all_wait(k_full(s), uint32_t(t / ST) & 1u, 64)) return false;
+      if (t > 0 && !all_wait(s_free, uint32_t(t - 1) & 1u, 67)) return false;
       tc::fence_after_sync();
       if (one) {
 #pragma unroll
@@ -249,150 +263,167 @@ flash_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
         }
         tc::mma_commit(s_full);
         tc::mma_commit(k_free(s));
+        if (last) tc::mma_commit(q_free);
       }
       __syncwarp();
       return true;
     };
-    if (n > 0) ok = scores(0);
-    for (int j = 0; j < n && ok; ++j) {
-      const int s = j % ST;
-      if (j + 1 < n) {
-        ok = __all_sync(0xffffffffu, wait(s_free, uint32_t(j) & 1u, p.status, 67));
-        if (ok) ok = scores(j + 1);
+    int t = 0, taken = 0;  // tiles and units with keys so far
+    for (int u = int(blockIdx.x); u < p.units && ok; u += step) {
+      const Unit w = unit(u);
+      if (w.n == 0) continue;
+      ok = all_wait(q_full, uint32_t(taken) & 1u, 71) && scores(t, w.n == 1);
+      for (int j = 0; j < w.n && ok; ++j, ++t) {
+        const int s = t % ST;
+        if (j + 1 < w.n) ok = scores(t + 1, j + 2 == w.n);
+        if (ok) ok = all_wait(v_full(s), uint32_t(t / ST) & 1u, 65);
         if (!ok) break;
-      }
-      ok = __all_sync(0xffffffffu, wait(v_full(s), uint32_t(j / ST) & 1u, p.status, 65));
-      if (!ok) break;
-      if (j == n - 1 && last_keys < kKeys) {  // values behind the last key may be anything, and their weights of zero would not silence a NaN
-        const uint32_t v = base + L::kV + uint32_t(s * L::kTile);
-        for (int x = 0; x < HALVES; ++x)
-          for (int i = last_keys * 8 + lane; i < kKeys * 8; i += 32) tc::st_shared_v4(v + uint32_t(x * kKeys * 128 + i * 16), 0, 0, 0, 0);
-        tc::fence_proxy_async_smem();
+        if (j == w.n - 1 && w.last_keys < kKeys) {  // values behind the last key may be anything, and their weights of zero would not silence a NaN
+          const uint32_t v = base + L::kV + uint32_t(s * L::kTile);
+          for (int x = 0; x < HALVES; ++x)
+            for (int i = w.last_keys * 8 + lane; i < kKeys * 8; i += 32) tc::st_shared_v4(v + uint32_t(x * kKeys * 128 + i * 16), 0, 0, 0, 0);
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (j == 0 && taken > 0) ok = all_wait(o_free, uint32_t(taken - 1) & 1u, 72);
+        if (ok) ok = all_wait(p_full, uint32_t(t) & 1u, 66);
+        if (!ok) break;
+        tc::fence_after_sync();
+        if (one) {
+#pragma unroll
+          for (int x = 0; x < kKeys / 16; ++x)
+            mma_f16_ts(tmem + kOut, tmem + kP + x * 8, smem_desc_mn_sw128(base + L::kV + uint32_t(s * L::kTile + x * 2048), kKeys * 128), o_desc, j != 0 || x != 0);
+          tc::mma_commit(o_done);
+          tc::mma_commit(v_free(s));
+        }
         __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, wait(p_full, uint32_t(j) & 1u, p.status, 66));
-      if (!ok) break;
-      tc::fence_after_sync();
-      if (one) {
-#pragma unroll
-        for (int x = 0; x < kKeys / 16; ++x)
-          mma_f16_ts(tmem + kOut, tmem + kP + x * 8, smem_desc_mn_sw128(base + L::kV + uint32_t(s * L::kTile + x * 2048), kKeys * 128), o_desc, j != 0 || x != 0);
-        tc::mma_commit(o_done);
-        tc::mma_commit(v_free(s));
-      }
-      __syncwarp();
+      ++taken;
     }
-  } else {
+  } else if (warp >= 2) {
     const int quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lanes = tmem + (uint32_t(quad * 32) << 16);
-    float m = -INFINITY, sum = 0.f;
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      ok = __all_sync(0xffffffffu, wait(s_full, uint32_t(j) & 1u, p.status, 68));
-      if (!ok) break;
-      tc::fence_after_sync();
-      uint32_t s[kKeys / 32][32];
+    int t = 0;
+    for (int u = int(blockIdx.x); u < p.units && ok; u += step) {
+      const Unit w = unit(u);
+      float m = -INFINITY, sum = 0.f;
+      for (int j = 0; j < w.n; ++j, ++t) {
+        ok = __all_sync(0xffffffffu, wait(s_full, uint32_t(t) & 1u, p.status, 68));
+        if (!ok) break;
+        tc::fence_after_sync();
+        uint32_t s[kKeys / 32][32];
 #pragma unroll
-      for (int x = 0; x < kKeys / 32; ++x) tc::tmem_ld_32x32(lanes + x * 32, s[x]);
-      tc::tmem_ld_wait();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(s_free);
-      if (j == n - 1 && last_keys < kKeys) {
+        for (int x = 0; x < kKeys / 32; ++x) tc::tmem_ld_32x32(lanes + x * 32, s[x]);
+        tc::tmem_ld_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(s_free);
+        if (j == w.n - 1 && w.last_keys < kKeys) {
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i)
-          if (i >= last_keys) s[i / 32][i % 32] = 0xff800000u;  // -inf
+          for (int i = 0; i < kKeys; ++i)
+            if (i >= w.last_keys) s[i / 32][i % 32] = 0xff800000u;  // -inf
+        }
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2) mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], __uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
+        const float high = fmaxf(mx[0], mx[1]) * p.scale_log2;
+        // the weights' columns, and the result, are this warp's again when the product before is done
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(t - 1) & 1u, p.status, 69));
+          if (!ok) break;
+          tc::fence_after_sync();
+        }
+        if (__any_sync(0xffffffffu, high > m + 8.f)) {
+          const float now = fmaxf(m, high);
+          if (j > 0) {
+            const float corr = m == now ? 1.f : ex2f(m - now);
+            sum *= corr;
+#pragma unroll
+            for (int x = 0; x < HD / 16; ++x) {
+              uint32_t o[16];
+              tc::tmem_ld_32x16(lanes + kOut + x * 16, o);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+              tmem_st_32x16(lanes + kOut + x * 16, o);
+            }
+          }
+          m = now;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const unsigned long long scale2 = two(p.scale_log2, p.scale_log2), less2 = two(-ref, -ref);
+        unsigned long long acc[2] = {0, 0};
+#pragma unroll
+        for (int x = 0; x < kKeys / 32; ++x) {
+          uint32_t w16[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            unsigned long long v = two(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1]));
+            asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(v) : "l"(scale2), "l"(less2));
+            if (i % 4 == 3) {
+              v = ex2_poly(v);
+            } else {
+              float lo, hi;
+              asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+              v = two(ex2f(lo), ex2f(hi));
+            }
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(v));
+            float lo, hi;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+            w16[i] = pack16<BF16>(lo, hi);
+          }
+          tmem_st_32x16(lanes + kP + x * 16, w16);
+        }
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[0]) : "l"(acc[1]));
+        float a0, a1;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc[0]));
+        sum += a0 + a1;
+        tc::tmem_st_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full);
       }
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < kKeys; i += 2) mx[(i >> 1) & 1] = max3(mx[(i >> 1) & 1], __uint_as_float(s[i / 32][i % 32]), __uint_as_float(s[i / 32][i % 32 + 1]));
-      const float high = fmaxf(mx[0], mx[1]) * p.scale_log2;
-      // the weights' columns, and the result, are this warp's again when the product before is done
-      if (j > 0) {
-        ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(j - 1) & 1u, p.status, 69));
+      if (!ok) break;
+      if (w.n > 0) {
+        ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(t - 1) & 1u, p.status, 70));
         if (!ok) break;
         tc::fence_after_sync();
       }
-      if (__any_sync(0xffffffffu, high > m + 8.f)) {
-        const float now = fmaxf(m, high);
-        if (j > 0) {
-          const float corr = m == now ? 1.f : ex2f(m - now);
-          sum *= corr;
+      if (m == -INFINITY && sum == sum) sum = 0.f;  // nothing above -inf
+      const int rr = w.row0 + r, token = p.G == 1 ? rr : rr / p.G;
+      float* to = w.rest >= 0 ? p.parts + size_t(w.rest) * part_floats(HD) : nullptr;
+      uint16_t* out = p.out + ((size_t(w.b) * p.R + token) * (p.Hkv * p.G) + w.h * p.G + rr - token * p.G) * HD;
+      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
-          for (int x = 0; x < HD / 16; ++x) {
-            uint32_t o[16];
-            tc::tmem_ld_32x16(lanes + kOut + x * 16, o);
-            tc::tmem_ld_wait();
+      for (int x = 0; x < HD / 32; ++x) {
+        uint32_t o[32];
+        if (w.n > 0) {
+          tc::tmem_ld_32x32(lanes + kOut + x * 32, o);
+          tc::tmem_ld_wait();
+        } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            tmem_st_32x16(lanes + kOut + x * 16, o);
-          }
+          for (int i = 0; i < 32; ++i) o[i] = 0;
         }
-        m = now;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      const unsigned long long scale2 = two(p.scale_log2, p.scale_log2), less2 = two(-ref, -ref);
-      unsigned long long acc[2] = {0, 0};
-#pragma unroll
-      for (int x = 0; x < kKeys / 32; ++x) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          unsigned long long v = two(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1]));
-          asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(v) : "l"(scale2), "l"(less2));
-          if (i % 4 == 3) {
-            v = ex2_poly(v);
-          } else {
-            float lo, hi;
-            asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-            v = two(ex2f(lo), ex2f(hi));
-          }
-          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(v));
-          float lo, hi;
-          asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-          w[i] = pack16<BF16>(lo, hi);
+        if (x == HD / 32 - 1 && w.n > 0) {  // the next unit's products may overwrite it
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(o_free);
         }
-        tmem_st_32x16(lanes + kP + x * 16, w);
+        if (r < w.rows && to) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(to + r * HD + x * 32 + i * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else if (r < w.rows) {
+          uint32_t w16[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w16[i] = pack16<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + x * 32 + i * 8) = make_uint4(w16[4 * i], w16[4 * i + 1], w16[4 * i + 2], w16[4 * i + 3]);
+        }
+        __syncwarp();
       }
-      asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[0]) : "l"(acc[1]));
-      float a0, a1;
-      asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc[0]));
-      sum += a0 + a1;
-      tc::tmem_st_wait();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(p_full);
+      if (to && r < w.rows) *reinterpret_cast<float2*>(to + kTcRows * HD + r * 2) = make_float2(m, sum);
     }
-    if (n > 0 && ok) ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(n - 1) & 1u, p.status, 70));
-    tc::fence_after_sync();
-    if (m == -INFINITY && sum == sum) sum = 0.f;  // nothing above -inf
-    const int rr = row0 + r;
-    float* to = p.parts && !alone ? p.parts + (size_t(rest / split) * p.slots + part) * part_floats(HD) : nullptr;
-    uint16_t* out = p.out + ((size_t(b) * p.R + rr / p.G) * (p.Hkv * p.G) + h * p.G + rr % p.G) * HD;
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int x = 0; x < HD / 32; ++x) {
-      uint32_t o[32];
-      if (n > 0 && ok) {
-        tc::tmem_ld_32x32(lanes + kOut + x * 32, o);
-        tc::tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0;
-      }
-      if (r < rows && to) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(to + r * HD + x * 32 + i * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-      } else if (r < rows) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack16<BF16>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + x * 32 + i * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      }
-      __syncwarp();
-    }
-    if (to && r < rows) *reinterpret_cast<float2*>(to + kTcRows * HD + r * 2) = make_float2(m, sum);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -485,10 +516,10 @@ int launch_behind(void (*kern)(Args...), int64_t blocks, int threads, size_t sme
 }
 
 template <int HD, bool BF16>
-int launch_flash(const CUtensorMap& kmap, const CUtensorMap& vmap, const FlashParams& p, int64_t items, cudaStream_t stream) {
+int launch_flash(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap, const FlashParams& p, int sm_count, cudaStream_t stream) {
   auto kern = flash_kernel<HD, BF16>;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), FlashLayout<HD>::kBytes);
-  return rc ? rc : launch_behind(kern, p.whole + (items - p.whole) * p.split, 192, FlashLayout<HD>::kBytes, stream, kmap, vmap, p);
+  return rc ? rc : launch_behind(kern, std::min(p.units, 2 * sm_count), 192, FlashLayout<HD>::kBytes, stream, qmap, kmap, vmap, p);
 }
 
 }  // namespace
@@ -508,28 +539,31 @@ int rows_attention_join(const RowsParams& r, int hd, bool bf16, int64_t B, int64
   return bf16 ? go(join_kernel<128, true, 8>, 1) : go(join_kernel<128, false, 8>, 1);
 }
 
-int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, cudaStream_t stream) {
+int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, int sm_count, cudaStream_t stream) {
   FlashParams p = {};
-  p.q = r.q, p.out = r.out, p.len = r.len;
+  p.out = r.out, p.len = r.len;
   p.parts = parts;
   p.status = static_cast<unsigned*>(status);
-  p.q_b = r.q_b, p.q_r = r.q_r, p.q_h = r.q_h, p.keys = r.keys;
+  p.keys = r.keys;
   p.R = r.R, p.G = r.G, p.Hkv = r.Hkv;
   p.tiles = (r.R * r.G + kTcRows - 1) / kTcRows;
   p.whole = int(plan.whole);
   p.split = plan.split;
   p.slots = plan.split + more;
-  p.scale_log2 = r.scale_log2 < 0.f ? -r.scale_log2 : r.scale_log2;
-  p.q_flip = r.scale_log2 < 0.f ? 0x80008000u : 0u;
+  p.scale_log2 = r.scale_log2;
   p.k_batch = r.k_b != 0, p.v_batch = r.v_b != 0, p.k_head = r.k_h != 0, p.v_head = r.v_h != 0;
   const uint32_t keys = hd == 64 ? FlashLayout<64>::kKeys : FlashLayout<128>::kKeys;
-  CUtensorMap kmap, vmap;
-  int rc = make_tmap_4d(&kmap, r.k, bf16, hd, uint64_t(r.keys), r.k_h ? r.Hkv : 1, r.k_b ? uint64_t(B) : 1, r.k_t, r.k_h, r.k_b, 64, keys);
-  if (!rc) rc = make_tmap_4d(&vmap, r.v, bf16, hd, uint64_t(r.keys), r.v_h ? r.Hkv : 1, r.v_b ? uint64_t(B) : 1, r.v_t, r.v_h, r.v_b, 64, keys);
+  CUtensorMap qmap, kmap, vmap;
+  const TmapDim q_dims[4] = {{uint64_t(p.G), r.q_h, uint32_t(p.G)}, {uint64_t(p.R), r.q_r, uint32_t(kTcRows / p.G)}, {uint64_t(p.Hkv), p.G * r.q_h, 1}, {uint64_t(B), r.q_b, 1}};
+  int rc = make_tmap_rows(&qmap, r.q, bf16, hd, 64, q_dims, 4);
+  const TmapDim k_dims[3] = {{uint64_t(r.keys), r.k_t, keys}, {r.k_h ? uint64_t(r.Hkv) : 1, r.k_h, 1}, {r.k_b ? uint64_t(B) : 1, r.k_b, 1}};
+  if (!rc) rc = make_tmap_rows(&kmap, r.k, bf16, hd, 64, k_dims, 3);
+  const TmapDim v_dims[3] = {{uint64_t(r.keys), r.v_t, keys}, {r.v_h ? uint64_t(r.Hkv) : 1, r.v_h, 1}, {r.v_b ? uint64_t(B) : 1, r.v_b, 1}};
+  if (!rc) rc = make_tmap_rows(&vmap, r.v, bf16, hd, 64, v_dims, 3);
   if (rc) return rc;
-  const int64_t items = B * p.Hkv * p.tiles;
-  if (hd == 64) return bf16 ? launch_flash<64, true>(kmap, vmap, p, items, stream) : launch_flash<64, false>(kmap, vmap, p, items, stream);
-  return bf16 ? launch_flash<128, true>(kmap, vmap, p, items, stream) : launch_flash<128, false>(kmap, vmap, p, items, stream);
+  p.units = int(plan.whole + (B * p.Hkv * p.tiles - plan.whole) * plan.split);
+  if (hd == 64) return bf16 ? launch_flash<64, true>(qmap, kmap, vmap, p, sm_count, stream) : launch_flash<64, false>(qmap, kmap, vmap, p, sm_count, stream);
+  return bf16 ? launch_flash<128, true>(qmap, kmap, vmap, p, sm_count, stream) : launch_flash<128, false>(qmap, kmap, vmap, p, sm_count, stream);
 }
 
 }  // namespace asrq

@@ -457,9 +457,13 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 enum TmapSwizzle { kSwizzleNone = 0, kSwizzle128 = 1, kSwizzle64 = 2 };
 int make_tmap_2d(CUtensorMap* out, const void* base, int elem_bytes, bool bf16, uint64_t inner, uint64_t rows,
                  uint32_t box_inner, uint32_t box_rows, TmapSwizzle swizzle);
-// 16-bit tensor of d3 x d2 x d1 x inner elements at strides of s3, s2, s1 elements (multiples of 8; any for a dimension of one), box 1 x 1 x box_1 x
-// box_inner, 128-byte swizzle, zero outside.
-int make_tmap_4d(CUtensorMap* out, const void* base, bool bf16, uint64_t inner, uint64_t d1, uint64_t d2, uint64_t d3, int64_t s1, int64_t s2, int64_t s3,
-                 uint32_t box_inner, uint32_t box_1);
+// 16-bit tensor: `inner` contiguous elements, then n (3 or 4) dimensions at strides in elements (multiples of 8; any for a dimension of one), box
+// box_inner elements x each dimension's, 128-byte swizzle, zero outside.
+struct TmapDim {
+  uint64_t size;
+  int64_t stride;
+  uint32_t box;
+};
+int make_tmap_rows(CUtensorMap* out, const void* base, bool bf16, uint64_t inner, uint32_t box_inner, const TmapDim* dims, int n);
 
 }  // namespace asrq
