@@ -6,7 +6,7 @@
 //   beam_reorder   cache[.., b * K + k, .., t] = cache[.., b * K + parent[b, k], .., t] for t < length, in place: bound by memory, the
 //                  rows that change written once and those they come from read once.
 //
-// The selection of an utterance is one cluster of 4 to 16 blocks and one launch, with no scratch in global memory, no counters
+// The selection of an utterance is one cluster of 2 to 16 blocks and one launch, with no scratch in global memory, no counters
 // that outlive the launch and no order of arrival in the result.  A warp reads a segment of one beam's row, 1024 values at a time:
 // each lane keeps the maximum and the sum of exponentials of its own values.  The warps of a block that share a row then agree on a value that
 // n of the lanes' maxima reach, and only the lanes whose maximum does (n of the row's lanes in the block, if maxima differ) are read again, by
@@ -16,7 +16,6 @@
 // sums.  Maxima, sums and lists go to the first block of the cluster, which joins the sums in 64 bits (the order of beams is decided by their
 // differences) and ranks what is no worse than a bound that n of the lists' best reach.
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -625,31 +624,6 @@ bool segments_fit(int64_t blocks, int64_t K, int64_t V) {
 }
 bool beam_select_fits(int64_t K, int64_t V) { return segments_fit(8, K, V); }
 
-// clusters of `blocks` that the chip holds at once
-int64_t select_clusters(int blocks, int sm_count) {
-  static std::atomic<int> known[17];  // one kind of device: asked once per process
-  int n = known[blocks].load(std::memory_order_relaxed);
-  if (n) return n;
-  cudaFuncSetAttribute(beam_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SelectShared)));
-  cudaFuncSetAttribute(beam_select_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks));
-  cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = sizeof(SelectShared);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(blocks);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, beam_select_kernel<false>, &cfg) != cudaSuccess || n < 1) {
-    cudaGetLastError();
-    n = std::max(1, sm_count / blocks);
-  }
-  known[blocks].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores, const uint8_t* finished, int64_t eos, float* out_scores,
                 long long* parents, long long* tokens, uint8_t* out_finished, int64_t B, int64_t K, int64_t V, int64_t n, int dtype, int sm_count,
                 cudaStream_t stream) {
@@ -670,9 +644,11 @@ int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores,
   auto kern = dtype == ASRQ_BF16 ? beam_select_kernel<true> : beam_select_kernel<false>;
   int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), sizeof(SelectShared));
   if (rc) return rc;
-  // As many blocks an utterance as the chip holds at once (64 utterances of 8 x 51866, us: 16 blocks @16, 8 @8, 4 @4).
+  // Blocks an utterance: a block an SM, two where that leaves four; the lists of two at least (us with 16 | 8 | 4 | 2: 1 utterance of 5 x 51866
+  // 9.5 | 11.4 | 12.8 | 16.9, 9 of them 12.0 | 11.8 | 13.4 | 17.5, 18 16.6 | 14.8 | 13.9 | 17.5, 32 23.7 | 18.4 | 14.9 | 18.5, 64 of 8 x 51866
+  // 52.6 | 34.4 | 25.1 | 28.7, 200 of 4 x 10000 88.6 | 46.4 | 26.2 | 18.3).
   int blocks = 16;
-  while (blocks > 4 && B > select_clusters(blocks, sm_count) && segments_fit(blocks / 2, K, V)) blocks /= 2;
+  while (blocks > 2 && B * blocks > (blocks == 4 ? 2 : 1) * sm_count && segments_fit(blocks / 2, K, V)) blocks /= 2;
   if (blocks > 8) ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(B * blocks));
