@@ -766,7 +766,7 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
   last_error().clear();
   if (!cache || !parents) return fail(ASRQ_ERR_NULL, "asrq_beam_reorder: cache and parents must not be NULL");
   if (L < 0 || B < 0 || K <= 0 || heads <= 0 || max_len <= 0 || position_bytes <= 0 || position_bytes % 16 || position_bytes > (1 << 20) ||
-      max_len > (int64_t(1) << 31) || L > (1 << 24) || B > (1 << 24) || heads > (1 << 16) || L * B > (1 << 30) || L * B * heads > 0x7fffffff)
+      max_len > (int64_t(1) << 31) || L > (1 << 24) || B > (1 << 24) || heads > (1 << 16) || L * B > (1 << 30) || L * B * heads > (1 << 30))
     return fail(ASRQ_ERR_SHAPE, "asrq_beam_reorder: L=%lld B=%lld K=%lld heads=%lld max_len=%lld position_bytes=%lld (a multiple of 16)", (long long)L,
                 (long long)B, (long long)K, (long long)heads, (long long)max_len, (long long)position_bytes);
   if (K > 32) return fail(ASRQ_ERR_LIMIT, "asrq_beam_reorder: K=%lld (at most 32)", (long long)K);
@@ -839,9 +839,10 @@ int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k
 
 size_t asrq_rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t shared_keys, int64_t own_keys) {
   const DeviceFacts* f;
-  if (B <= 0 || R <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || (head_dim != 64 && head_dim != 128) || shared_keys < 0 || own_keys < 0 ||
-      device_facts(&f))
-    return 0;
+  if (B <= 0 || R <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % n_kv_heads || n_q_heads > (1 << 16) || (head_dim != 64 && head_dim != 128) ||
+      shared_keys < 0 || own_keys < 0 || shared_keys > 0x7fffffff || own_keys > 0x7fffffff || R > (1 << 24) || B > (1 << 24) ||
+      R * (n_q_heads / n_kv_heads) > (1 << 24) || B * n_kv_heads * ((R * (n_q_heads / n_kv_heads) + 15) / 16) > (1 << 27) || device_facts(&f))
+    return 0;  // (no call of these sizes)
   return rows_attention_scratch_bytes(B, R, n_q_heads, n_kv_heads, head_dim, shared_keys, own_keys, f->sm_count);
 }
 

@@ -476,13 +476,14 @@ template <int HD, int MT, bool BF16>
 RowsChoice choose_rows(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys, int64_t keys2, int sm_count) {
   constexpr int ROWS = 16 * MT, KC = HD == 64 ? 32 : 16;
   const int64_t items = B * n_kv_heads * ((R * G + ROWS - 1) / ROWS);
-  const int64_t chunks = (keys + KC - 1) / KC + std::min<int64_t>((ROWS - 1) / G + 1, R) * ((keys2 + KC - 1) / KC);
+  // (32-bit divisions: the loop is host time of every call)
+  const uint32_t blocks = uint32_t(items), chunks = uint32_t(std::min<int64_t>((keys + KC - 1) / KC + std::min<int64_t>((ROWS - 1) / G + 1, R) * ((keys2 + KC - 1) / KC), 1 << 30));
   RowsChoice best = {1, kRowsWarps, INT64_MAX};
-  for (int s = 1; s <= kMaxSplit; s *= 2)
-    for (int w = kRowsWarps; w >= 1; --w) {
-      const int64_t slots = resident_blocks<HD, MT, BF16>(s, w, sm_count);
-      const int64_t cost = (items * s + slots - 1) / slots * ((chunks + s * w - 1) / (s * w) + (s > 1 ? 4 : 3));
-      if (cost < best.cost) best = {s, w, cost};
+  for (uint32_t s = 1; s <= uint32_t(kMaxSplit); s *= 2)
+    for (uint32_t w = kRowsWarps; w >= 1; --w) {
+      const uint32_t slots = uint32_t(resident_blocks<HD, MT, BF16>(int(s), int(w), sm_count));
+      const int64_t cost = int64_t((blocks * s + slots - 1) / slots) * ((chunks + s * w - 1) / (s * w) + (s > 1 ? 4 : 3));
+      if (cost < best.cost) best = {int(s), int(w), cost};
     }
   return best;
 }
@@ -502,8 +503,6 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
   p.tiles = (p.R * p.G + ROWS - 1) / ROWS;
   const int64_t items = B * p.Hkv * p.tiles;
   auto kern = rows_attn_kernel<HD, MT, BF16>;
-  const int rc = allow_rows<HD, MT, BF16>();
-  if (rc) return rc;
   const RowsChoice choice = choose_rows<HD, MT, BF16>(B, p.R, p.G, p.Hkv, p.keys, p.k2 ? p.keys2 : 0, sm_count);
   const int split = choice.split, warps = choice.warps;
   const size_t smem = rows_smem<HD, MT>(warps);
@@ -533,35 +532,46 @@ double rows_estimate(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_
   return 1.2 * double(choose_rows<64, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
 }
 
-// Whether the tensor-core kernel takes a call, and how it divides it.  It walks tiles of keys at 1.3 us a wave of blocks, with 3 for a block's start
-// and end, however few of the 128 rows there are; items that fill the chip are left whole, the rest divided so that it is filled once
-// more, and a join is worth about 4.  us, the row kernel first: heads of 64 on 1500 keys, 16 utterances of 5 rows 23 | 34, 20 rows 45 | 37, 64 rows
-// 76 | 38; 4 utterances of 32 rows 16 | 18, 40 rows 24 | 18; 1 of 64 11 | 14; heads of 128 on 6000 keys, 16 utterances of 20 rows 78 | 73, 64 rows 164 | 79.
+// Whether the tensor-core kernel takes a call, and how it divides it.  Its blocks walk tiles of keys at about 1.15 us each (1.3 where own keys follow),
+// one more for a unit of work and two for the start, however few of the 128 rows there are; items that fill the chip are left whole, the rest
+// divided so that it is filled once more, and a join is worth about 4.  us, the row kernel first: heads of 64 on 1500 keys, 16 utterances of 5 rows
+// 23 | 29, 20 rows 44 | 29, 64 rows 74 | 30; 4 of 32 rows 14 | 17, 64 rows 22 | 18; 1 of 64 rows 11 | 10; on 150 keys, 16 of 20 rows 10.7 | 8.7, of 5 5.4 | 8.7;
+// heads of 128 on 6000 keys, 16 utterances of 8 rows 64 | 74, 20 rows 107 | 76, 64 rows 279 | 84; behind 6000 shared keys 200 own ones, 4 utterances of 16
+// beams 34 | 41, 32 beams 56 | 51.
 TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
   const int64_t rows = R * G, tiles = (rows + kTcRows - 1) / kTcRows, items = B * n_kv_heads * tiles, step = hd == 64 ? 96 : 64;
   const int64_t key_tiles = (keys + step - 1) / step, slots = 2 * sm_count;
   const bool own = keys2 > 0;
   const int forced = option(kOptRowsKernel);
   if (keys == 0 || kTcRows % G != 0 || forced == 1 || (forced != 2 && (rows <= 16 || keys < 64))) return {0, 0};
-  const int64_t whole = own ? 0 : items / slots * slots, rest = items - whole, first = whole / slots * (key_tiles + 3);
+  const int64_t whole = own ? 0 : items / slots * slots, rest = items - whole, first = whole / slots * (key_tiles + 1);
   TcPlan plan = {own ? 0 : items, own ? 0 : 1};
-  int64_t least = rest == 0 ? 0 : own ? INT64_MAX : key_tiles + 3;
+  int64_t least = rest == 0 ? 0 : own ? INT64_MAX : key_tiles + 1;
   for (int s = own ? 1 : 2; s <= kMaxParts && rest > 0 && (s == 1 || key_tiles >= 2 * s); ++s) {
-    const int64_t cost = (rest * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 3) + 4 + s / 8;
+    const int64_t cost = (rest * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 1) + 4 + s / 8;
     if (cost < least) {
       least = cost;
       plan = {whole, s};
     }
   }
   if (forced == 2) return plan;
-  double us = 1.3 * double(first + least);
+  double us = (own ? 1.3 : 1.15) * double(first + least + 2);
   if (own) us += rows_estimate(B, R, G, n_kv_heads, hd, 0, keys2, sm_count);
   return us < rows_estimate(B, R, G, n_kv_heads, hd, keys, keys2, sm_count) ? plan : TcPlan{0, 0};
 }
 int allow_all() {
+  static std::atomic<uint64_t> devices;  // that have it
+  int dev = 0;
+  ASRQ_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (devices.load(std::memory_order_relaxed) & bit) return ASRQ_OK;
   int rc = allow_rows<64, 1, false>();
+  if (!rc) rc = allow_rows<64, 1, true>();
   if (!rc) rc = allow_rows<64, 2, false>();
+  if (!rc) rc = allow_rows<64, 2, true>();
   if (!rc) rc = allow_rows<128, 1, false>();
+  if (!rc) rc = allow_rows<128, 1, true>();
+  if (!rc) devices.fetch_or(bit, std::memory_order_relaxed);
   return rc;
 }
 size_t part_bytes(int64_t B, int64_t R, int G, int n_kv_heads, int hd, const TcPlan& plan, bool own) {

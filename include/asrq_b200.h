@@ -312,8 +312,8 @@ int asrq_decode_grouped_attention(const void* qkv, const void* q_weight, const v
  *   logits      beam k of utterance b at logits + b * utterance_stride + k * beam_stride, V contiguous values of `dtype`, at any value's address;
  *   scores      B x K; a beam whose score is not finite is no hypothesis: its continuations have -inf (at the first step all but one beam);
  *               so has one whose logits hold a NaN, a +inf or nothing above -inf;
- *   finished    B x K bytes, or NULL: a beam that has ended goes on with the token eos at its own score and with nothing else (-inf); its logits are not
- *               read.  out_finished (B x n): 1 where the parent had ended or the token is eos;
+ *   finished    B x K bytes, or NULL: a beam that has ended goes on with the token eos at its own score and with nothing else (-inf); its logits do
+ *               not matter.  out_finished (B x n): 1 where the parent had ended or the token is eos;
  *   out_scores, parents, tokens   B x n.
  * K and n at most 32, V at most 65536 * floor(128 / K).  No scratch, no state between calls.
  */
