@@ -136,6 +136,55 @@ __device__ __forceinline__ uint4 eight_of(const uint16_t* row, int e, int V, uin
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Vectors a and b of a row, eight values each, -inf past the row's end and in vectors from v1 on; the whole warp calls it.  The row may start at
+// any value: a vector is two aligned ones, shifted together.  Those that lie inside the row are all on their way before the first is looked
+// at, the two that its ends cut come value by value, a lane each.
+struct TwoVectors {
+  uint4 a, b;
+};
+template <bool bf16>
+__device__ __forceinline__ TwoVectors vectors_of(const uint16_t* row, int va, int vb, int v1, int V) {
+  constexpr uint32_t kNone = bf16 ? 0xff80u : 0xfc00u, kNone2 = kNone * 0x10001u;
+  const int off = int(uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u) / 2, lane = threadIdx.x & 31;
+  uint4 a[4];
+  int first[4];
+  bool wanted[4], cut = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int v = i < 2 ? va : vb;
+    first[i] = (v + (i & 1)) * 8 - off;
+    wanted[i] = v < v1 && (i % 2 == 0 || off != 0) && first[i] < V;
+    a[i] = make_uint4(kNone2, kNone2, kNone2, kNone2);
+    const bool in = first[i] >= 0 && first[i] + 8 <= V;
+    if (wanted[i] && in) a[i] = ld_x4(row + first[i]);
+    wanted[i] = wanted[i] && !in;
+    cut |= wanted[i];
+  }
+  if (__any_sync(0xffffffffu, cut)) {
+    const int last = (V - 1 + off) / 8, e = (lane < 8 ? 0 : last) * 8 + (lane & 7) - off;
+    uint32_t x = lane < 16 && e >= 0 && e < V ? ld_x1(row + e) : kNone;
+    x |= __shfl_down_sync(0xffffffffu, x, 1) << 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int from = first[i] <= 0 ? 0 : 8;
+      const uint4 end = make_uint4(__shfl_sync(0xffffffffu, x, from), __shfl_sync(0xffffffffu, x, from + 2), __shfl_sync(0xffffffffu, x, from + 4),
+                                   __shfl_sync(0xffffffffu, x, from + 6));
+      if (wanted[i]) a[i] = end;
+    }
+  }
+  auto shifted = [&](const uint4& lo, const uint4& hi) {
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int j = 0; j < 6; ++j) w[j] = off & 4 ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = off & 2 ? w[j + 1] : w[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 1) * 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  return {shifted(a[0], a[1]), shifted(a[2], a[3])};
+}
+
 // Candidates of an utterance: a larger key first, of equals the smaller place (beam * V + token)
 struct __align__(16) Cand {
   unsigned long long key;  // 0: none
@@ -177,6 +226,18 @@ __device__ __forceinline__ uint32_t best_of(uint32_t a, uint32_t b, int n, int l
   return out;
 }
 
+// The n-th largest of a warp's 16-bit words; a sort for many (about the time of 12 maxima)
+__device__ __forceinline__ uint32_t nth_of(uint32_t v, int n, int lane) {
+  if (n > 12) return __shfl_sync(0xffffffffu, sort_descending(v, lane), n - 1);
+  uint32_t key = v << 5 | uint32_t(lane), m = 0;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    m = __reduce_max_sync(0xffffffffu, key);
+    if (key == m) key = 0;
+  }
+  return m >> 5;
+}
+
 struct SelectShared {  // of the first block, but for floors
   uint32_t floors[kSelWarps][8];     // each block: a warp's largest lane maxima
   uint8_t order[kSelWarps][32];      // each block: the lanes that a warp reads again
@@ -211,7 +272,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
   const volatile uint8_t* over = p.finished ? p.finished + size_t(b) * K : nullptr;
   const int nvec = (V + 7) / 8, n_lists = int(blocks) * kSelWarps, id = int(rank) * kSelWarps + warp;
   uint32_t y[kSelWords];  // the next values
-  auto load = [&](const uint16_t* r, int vb, int v1) {
+  // (at_first: before the loop, where a row's ends may take registers; 1 utterance of 5 x 51866 values 9.1 -> 8.5 us)
+  auto load = [&](const uint16_t* r, int vb, int v1, auto at_first) {
     const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(r)) & 15u;
     if (vb > 0 && vb + 32 * kSelVecs <= v1 && (vb + 32 * kSelVecs + 1) * 8 <= V) {  // all of it and its neighbours inside the row
       const uint16_t* lo = r + size_t(vb + lane) * 8 - off / 2;
@@ -241,11 +303,20 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
       }
       return;
     }
+    if constexpr (decltype(at_first)::value) {
 #pragma unroll
-    for (int i = 0; i < kSelVecs; ++i) {
-      const int v = vb + i * 32 + lane;
-      const uint4 u = v < v1 ? eight_of(r, v * 8, V, kNone) : make_uint4(kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u);
-      y[4 * i] = u.x, y[4 * i + 1] = u.y, y[4 * i + 2] = u.z, y[4 * i + 3] = u.w;
+      for (int h = 0; h < kSelVecs; h += 2) {
+        const TwoVectors u = vectors_of<bf16>(r, vb + h * 32 + lane, vb + h * 32 + 32 + lane, v1, V);
+        y[4 * h] = u.a.x, y[4 * h + 1] = u.a.y, y[4 * h + 2] = u.a.z, y[4 * h + 3] = u.a.w;
+        y[4 * h + 4] = u.b.x, y[4 * h + 5] = u.b.y, y[4 * h + 6] = u.b.z, y[4 * h + 7] = u.b.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSelVecs; ++i) {
+        const int v = vb + i * 32 + lane;
+        const uint4 u = v < v1 ? eight_of(r, v * 8, V, kNone) : make_uint4(kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u, kNone * 0x10001u);
+        y[4 * i] = u.x, y[4 * i + 1] = u.y, y[4 * i + 2] = u.z, y[4 * i + 3] = u.w;
+      }
     }
   };
   const float early = warp == 0 && lane < K ? scores[lane] : 0.f;
@@ -254,7 +325,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
   const int guess_per_row = n_lists / K, guess_row = id / guess_per_row;
   if (guess_row < K) {
     const int seg_vecs = (nvec + guess_per_row - 1) / guess_per_row, v0 = (id - guess_row * guess_per_row) * seg_vecs, v1 = min(nvec, v0 + seg_vecs);
-    if (v0 < v1) load(p.logits + size_t(b) * p.sb + size_t(guess_row) * p.sk, v0, v1);
+    if (v0 < v1) load(p.logits + size_t(b) * p.sb + size_t(guess_row) * p.sk, v0, v1, std::true_type{});
   }
   if (warp == 0) {
     int state = kRowNone;
@@ -281,7 +352,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
   double sum = 0.0;            // of exp(x - top), this lane's
   uint32_t mine = kNone * 0x10001u;  // this lane's maximum, of low and high halves
   if (works) {
-    if (!(row_id == guess_row && n_live == K)) load(r, v0, v1);
+    if (!(row_id == guess_row && n_live == K)) load(r, v0, v1, std::false_type{});
 #pragma unroll 1
     for (int vb = v0; vb < v1; vb += 32 * kSelVecs) {
       uint32_t x[kSelWords], mx = y[0];
@@ -289,7 +360,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
       for (int i = 0; i < kSelWords; ++i) x[i] = y[i];
 #pragma unroll
       for (int i = 1; i < kSelWords; ++i) mx = max2<bf16>(mx, x[i]);
-      if (vb + 32 * kSelVecs < v1) load(r, vb + 32 * kSelVecs, v1);
+      if (vb + 32 * kSelVecs < v1) load(r, vb + 32 * kSelVecs, v1, std::false_type{});
       mine = max2<bf16>(mine, mx);
       // (a NaN may pass as any maximum here: the row is no distribution then)
       const float lane_top = fmaxf(out16_to_float(uint16_t(mine & 0xffffu), bf16), out16_to_float(uint16_t(mine >> 16), bf16)), ref = lane_top > -INFINITY ? lane_top : 0.f;
@@ -310,25 +381,36 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_select_kernel(const Selec
   const float lo = out16_to_float(uint16_t(mine & 0xffffu), bf16), hi = out16_to_float(uint16_t(mine >> 16), bf16);
   const bool bad = __any_sync(0xffffffffu, !(fmaxf(lo, hi) < INFINITY) || lo != lo || hi != hi);
   const uint32_t best = ordered16(lo >= hi ? mine & 0xffffu : mine >> 16);  // this lane's largest
-  const uint32_t by_lane = sort_descending(best, lane);
+  // the largest few of the lanes' for the block: of its warps on this row, 32 values at most
+  const int w0 = max(warp - seg, 0), w1 = min(warp + per_row - seg, kSelWarps), each = min(8, 32 / (w1 - w0));
+  const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+  {
+    uint32_t key = best << 5 | uint32_t(lane);
+#pragma unroll 1
+    for (int i = 0; i < each; ++i) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, key);
+      if (key == m) key = 0;
+      if (lane == 0) sh.floors[warp][i] = m >> 5;
+    }
+  }
   {  // from the lanes' maxima to the warp's
-    const float all = out16_to_float(unordered16(__shfl_sync(0xffffffffu, by_lane, 0)), bf16);
+    const float all = out16_to_float(unordered16(most), bf16);
     if (top > -INFINITY) sum *= double(exp2_fast((top - all) * kLog2e));
     top = bad ? INFINITY : all;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if (lane < 8) sh.floors[warp][lane] = by_lane;
   __syncthreads();
   uint32_t list = 0;  // this lane's entry of the warp's list
   if (works && !bad) {
     uint32_t last = 0;  // n entries are no worse
     // n values of the row are at least `least`: of this warp's lanes, or of the first few of each of the block's warps on this row
-    uint32_t least = __shfl_sync(0xffffffffu, by_lane, n - 1);
-    const int w0 = max(warp - seg, 0), w1 = min(warp + per_row - seg, kSelWarps), each = min(8, 32 / (w1 - w0));
+    uint32_t least;
     if (each * (w1 - w0) >= n) {
       const uint32_t at = lane < each * (w1 - w0) ? *(const volatile uint32_t*)&sh.floors[w0 + lane / each][lane % each] : 0u;
-      least = max(least, __shfl_sync(0xffffffffu, sort_descending(at, lane), n - 1));
+      least = nth_of(at, n, lane);
+    } else {
+      least = nth_of(best, n, lane);
     }
     const uint32_t least2 = uint32_t(unordered16(least)) * 0x10001u;
     int waiting = 0;  // entries so far, at most 32, in no order
@@ -645,8 +727,8 @@ int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores,
   int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), sizeof(SelectShared));
   if (rc) return rc;
   // Blocks an utterance: a block an SM, two where that leaves four; the lists of two at least (us with 16 | 8 | 4 | 2: 1 utterance of 5 x 51866
-  // 9.5 | 11.4 | 12.8 | 16.9, 9 of them 12.0 | 11.8 | 13.4 | 17.5, 18 16.6 | 14.8 | 13.9 | 17.5, 32 23.7 | 18.4 | 14.9 | 18.5, 64 of 8 x 51866
-  // 52.6 | 34.4 | 25.1 | 28.7, 200 of 4 x 10000 88.6 | 46.4 | 26.2 | 18.3).
+  // 8.2 | 10.4 | 11.9 | 16.2, 9 of them 10.5 | 10.5 | 12.4 | 17.0, 18 14.6 | 13.2 | 12.4 | 17.5, 32 20.6 | 16.7 | 14.1 | 17.8, 64 of 8 x 51866
+  // 53.4 | 34.7 | 24.0 | 29.4, 200 of 4 x 10000 93.9 | 47.8 | 26.5 | 18.2).
   int blocks = 16;
   while (blocks > 2 && B * blocks > (blocks == 4 ? 2 : 1) * sm_count && segments_fit(blocks / 2, K, V)) blocks /= 2;
   if (blocks > 8) ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
