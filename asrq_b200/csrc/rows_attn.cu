@@ -534,7 +534,7 @@ double rows_estimate(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_
 
 // Whether the tensor-core kernel takes a call, and how it divides it.  Its blocks walk tiles of keys at about 1.15 us each (1.3 where own keys follow),
 // one more for a unit of work and two for the start, however few of the 128 rows there are; items that fill the chip are left whole, the rest
-// divided so that it is filled once more, and a join is worth about 4.  us, the row kernel first: heads of 64 on 1500 keys, 16 utterances of 5 rows
+// divided so that it is filled once more, and a join is worth about 4, of up to 64 rows of 128 dimensions 3.  us, the row kernel first: heads of 64 on 1500 keys, 16 utterances of 5 rows
 // 23 | 29, 20 rows 44 | 29, 64 rows 74 | 30; 4 of 32 rows 14 | 17, 64 rows 22 | 18; 1 of 64 rows 11 | 10; on 150 keys, 16 of 20 rows 10.7 | 8.7, of 5 5.4 | 8.7;
 // heads of 128 on 6000 keys, 16 utterances of 8 rows 64 | 74, 20 rows 107 | 76, 64 rows 279 | 84; behind 6000 shared keys 200 own ones, 4 utterances of 16
 // beams 34 | 41, 32 beams 56 | 51.
@@ -548,7 +548,7 @@ TcPlan tc_plan(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys
   TcPlan plan = {own ? 0 : items, own ? 0 : 1};
   int64_t least = rest == 0 ? 0 : own ? INT64_MAX : key_tiles + 1;
   for (int s = own ? 1 : 2; s <= kMaxParts && rest > 0 && (s == 1 || key_tiles >= 2 * s); ++s) {
-    const int64_t cost = (rest * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 1) + 4 + s / 8;
+    const int64_t cost = (rest * s + slots - 1) / slots * ((key_tiles + s - 1) / s + 1) + (hd == 128 && rows <= 64 ? 3 : 4) + s / 8;
     if (cost < least) {
       least = cost;
       plan = {whole, s};
