@@ -770,7 +770,7 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
     return fail(ASRQ_ERR_SHAPE, "asrq_beam_reorder: L=%lld B=%lld K=%lld heads=%lld max_len=%lld position_bytes=%lld (a multiple of 16)", (long long)L,
                 (long long)B, (long long)K, (long long)heads, (long long)max_len, (long long)position_bytes);
   if (K > 32) return fail(ASRQ_ERR_LIMIT, "asrq_beam_reorder: K=%lld (at most 32)", (long long)K);
-  if (!aligned16(cache)) return fail(ASRQ_ERR_ALIGN, "asrq_beam_reorder: cache must be 16-byte aligned");
+  if (!aligned16(cache) || !aligned16(workspace)) return fail(ASRQ_ERR_ALIGN, "asrq_beam_reorder: cache and workspace must be 16-byte aligned");
   if (!workspace || workspace_bytes < kStatusBytes) return fail(ASRQ_ERR_WORKSPACE, "asrq_beam_reorder: workspace");
   const DeviceFacts* f;
   int rc;
@@ -783,7 +783,7 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
 namespace {
 // What the two attentions of shared keys have in common
 int check_rows(const char* who, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* out, int64_t B,
-               int64_t R, int nq, int nkv, int hd, int64_t keys, int dtype, const void* scratch) {
+               int64_t R, int nq, int nkv, int hd, int64_t keys, int dtype, const void* workspace, const void* scratch) {
   if (!q || !out || !qs || !ks || !vs || (keys > 0 && (!k || !v))) return fail(ASRQ_ERR_NULL, "%s: q, k, v, out and the strides must not be NULL", who);
   if (dtype != ASRQ_F16 && dtype != ASRQ_BF16) return fail(ASRQ_ERR_DTYPE, "%s: dtype %d", who, dtype);
   if (B < 0 || R < 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq > (1 << 16) || (hd != 64 && hd != 128) || keys < 0 || keys > 0x7fffffff || R > (1 << 24) ||
@@ -792,9 +792,8 @@ int check_rows(const char* who, const void* q, const int64_t* qs, const void* k,
   for (const int64_t* s : {qs, ks, vs})
     if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[0] % 8 || s[1] % 8 || s[2] % 8)
       return fail(ASRQ_ERR_ALIGN, "%s: strides %lld, %lld, %lld (multiples of 8)", who, (long long)s[0], (long long)s[1], (long long)s[2]);
-  if (scratch && !aligned16(scratch)) return fail(ASRQ_ERR_ALIGN, "%s: scratch must be 16-byte aligned", who);
-  for (const void* x : {q, keys > 0 ? k : q, keys > 0 ? v : q})
-    if (!aligned16(x)) return fail(ASRQ_ERR_ALIGN, "%s: q, k and v must be 16-byte aligned", who);
+  for (const void* x : {q, keys > 0 ? k : q, keys > 0 ? v : q, out, workspace, scratch})  // (NULL is aligned)
+    if (!aligned16(x)) return fail(ASRQ_ERR_ALIGN, "%s: q, k, v, out, workspace and scratch must be 16-byte aligned", who);
   return ASRQ_OK;
 }
 }  // namespace
@@ -803,7 +802,7 @@ int asrq_cross_attention(const void* q, const int64_t* q_strides, const void* k,
                          const int64_t* lengths, void* out, int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int head_dim, int64_t keys, float scale,
                          int dtype, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
   last_error().clear();
-  int rc = check_rows("asrq_cross_attention", q, q_strides, k, k_strides, v, v_strides, out, B, R, n_q_heads, n_kv_heads, head_dim, keys, dtype, scratch);
+  int rc = check_rows("asrq_cross_attention", q, q_strides, k, k_strides, v, v_strides, out, B, R, n_q_heads, n_kv_heads, head_dim, keys, dtype, workspace, scratch);
   if (rc) return rc;
   const DeviceFacts* f;
   if ((rc = device_facts(&f))) return rc;
@@ -820,10 +819,10 @@ int asrq_prefix_attention(const void* q, const int64_t* q_strides, const void* k
                           void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes, void* stream) {
   last_error().clear();
   int rc = check_rows("asrq_prefix_attention", q, q_strides, k_prefix, k_prefix_strides, v_prefix, v_prefix_strides, out, B, K, n_q_heads, n_kv_heads, head_dim,
-                      prefix_keys, dtype, scratch);
+                      prefix_keys, dtype, workspace, scratch);
   if (!rc)
     rc = check_rows("asrq_prefix_attention", q, q_strides, k_suffix, k_suffix_strides, v_suffix, v_suffix_strides, out, B, K, n_q_heads, n_kv_heads, head_dim,
-                    suffix_keys, dtype, scratch);
+                    suffix_keys, dtype, workspace, scratch);
   if (rc) return rc;
   if (!suffix_lengths) return fail(ASRQ_ERR_NULL, "asrq_prefix_attention: suffix_lengths must not be NULL");
   if (n_suffix_lengths != 1 && n_suffix_lengths != B * K)

@@ -326,7 +326,7 @@ int asrq_beam_select(const void* logits, int64_t utterance_stride, int64_t beam_
  * h < heads and the positions t < length, in place; positions from `length` on stay as they are.  cache: L x (B * K) x heads x max_len
  * positions of position_bytes (a multiple of 16), any type, 16-byte aligned.  parents: B x K; a parent outside 0..K-1 leaves its beam as it is.
  * The length is read from length_device when that is not NULL and is the argument otherwise, and is cut to 0..max_len.  K at most 32.
- * workspace: at least 256 bytes, the status block of any workspace (the kernel's waits are bounded; asrq_check_status).
+ * workspace: at least 256 bytes, 16-byte aligned, the status block of any workspace (the kernel's waits are bounded; asrq_check_status).
  * A kernel that reads the cache ahead of the stream dependency (asrq_decode_self_attention_settled,
  * asrq_decode_grouped_attention) needs an ordinary kernel or copy between this call and its own.
  */
@@ -339,7 +339,7 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
  *   q, q_strides   values between utterances, rows and heads;  k, v and theirs: between utterances, heads and positions; multiples of 8;
  *   lengths        B, cut to 0..keys, or NULL for `keys` everywhere; nothing past an utterance's length is read; a row without keys is zero;
  *   out            B x R x n_q_heads x head_dim, contiguous.
- * head_dim 64 or 128; q, k and v 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation; the weights are
+ * head_dim 64 or 128; q, k, v, out, workspace and scratch 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation; the weights are
  * rounded to `dtype`.
  * Many rows run on the tensor-core kernel, whose waits are bounded: it reports in the workspace's status block (256 bytes, the start of any workspace;
  * asrq_check_status) and, where it divides the keys or the rows have keys of their own, leaves parts in scratch of the call's own
