@@ -22,7 +22,7 @@ NATIVE = os.path.join(PKG, "_native.so")  # the module calls' host path (csrc/ho
 OBJ_DIR = os.path.join(PKG, "build")
 
 SOURCES = ["api.cu", "gemv_a16.cu", "gemv_a16_splitk.cu", "gemv_a16_staged.cu", "gemm_a16_tc.cu", "gemm_a16_tc2.cu", "gemm_a16_dense.cu", "gemm_a16_skinny.cu", "act_quant.cu", "glue.cu", "offline.cu", "dense_head.cu", "decode_attn.cu", "conformer.cu", "beam.cu", "rows_attn.cu", "rows_attn_tc.cu", "w4a4_mma.cu", "w4a4_tc.cu"]
-HEADERS = ["common.cuh", "tcgen05.cuh", "dequant.cuh", "rows_attn.cuh", os.path.join("..", "..", "include", "asrq_b200.h")]
+HEADERS = ["common.cuh", "tcgen05.cuh", "dequant.cuh", "rows_attn.cuh", "cluster_choice.h", os.path.join("..", "..", "include", "asrq_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -16,8 +16,10 @@
 // sums.  Maxima, sums and lists go to the first block of the cluster, which joins the sums in 64 bits (the order of beams is decided by their
 // differences) and ranks what is no worse than a bound that n of the lists' best reach.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
+#include "cluster_choice.h"
 #include "tcgen05.cuh"
 
 namespace asrq {
@@ -704,6 +706,36 @@ bool segments_fit(int64_t blocks, int64_t K, int64_t V) {
   const int64_t per_row = blocks * kSelWarps / K;
   return per_row > 0 && ((V + 7) / 8 + per_row - 1) / per_row * 8 <= kSegValues;
 }
+// Whether the current device holds clusters of 16 blocks of the selection: asked once for each device and kernel, which the answer also allows them
+int holds_clusters_of_16(void (*kern)(SelectParams), bool bf16, bool* holds) {
+  static std::atomic<uint64_t> asked[2], held[2];  // by device
+  int dev = 0;
+  ASRQ_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(asked[bf16].load(std::memory_order_acquire) & bit)) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = sizeof(SelectShared);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    if (n > 0) held[bf16].fetch_or(bit, std::memory_order_relaxed);
+    asked[bf16].fetch_or(bit, std::memory_order_release);
+  }
+  *holds = (held[bf16].load(std::memory_order_relaxed) & bit) != 0;
+  return ASRQ_OK;
+}
+
 bool beam_select_fits(int64_t K, int64_t V) { return segments_fit(8, K, V); }
 
 int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores, const uint8_t* finished, int64_t eos, float* out_scores,
@@ -726,12 +758,9 @@ int beam_select(const void* logits, int64_t sb, int64_t sk, const float* scores,
   auto kern = dtype == ASRQ_BF16 ? beam_select_kernel<true> : beam_select_kernel<false>;
   int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), sizeof(SelectShared));
   if (rc) return rc;
-  // Blocks an utterance: a block an SM, two where that leaves four; the lists of two at least (us with 16 | 8 | 4 | 2: 1 utterance of 5 x 51866
-  // 8.2 | 10.4 | 11.9 | 16.2, 9 of them 10.5 | 10.5 | 12.4 | 17.0, 18 14.6 | 13.2 | 12.4 | 17.5, 32 20.6 | 16.7 | 14.1 | 17.8, 64 of 8 x 51866
-  // 53.4 | 34.7 | 24.0 | 29.4, 200 of 4 x 10000 93.9 | 47.8 | 26.5 | 18.2).
-  int blocks = 16;
-  while (blocks > 2 && B * blocks > (blocks == 4 ? 2 : 1) * sm_count && segments_fit(blocks / 2, K, V)) blocks /= 2;
-  if (blocks > 8) ASRQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  bool holds_16 = false;
+  if ((rc = holds_clusters_of_16(kern, dtype == ASRQ_BF16, &holds_16))) return rc;
+  const int blocks = choose_select(B, sm_count, holds_16, [&](int n) { return segments_fit(n, K, V); });
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(B * blocks));
   cfg.blockDim = dim3(kSelThreads);

@@ -20,6 +20,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "cluster_choice.h"
 #include "rows_attn.cuh"
 
 namespace asrq {
@@ -27,9 +28,6 @@ namespace asrq {
 int ensure_dynamic_smem(const void* kernel, size_t bytes);
 
 namespace {
-
-constexpr int kRowsWarps = 8;
-constexpr int kMaxSplit = 16;  // blocks of a cluster
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -439,13 +437,13 @@ size_t rows_smem(int warps) {
   return size_t(warps) * kStages * kChunkBytes + (ROWS * HD + 2 * kMaxSplit * ROWS + 2 * ROWS) * 4;
 }
 
-// Blocks of `warps` warps, in clusters of `split`, that the device holds at once
+// Blocks of `warps` warps, in clusters of `split`, that the device holds at once; 0: it holds no such cluster
 template <int HD, int MT, bool BF16>
 int64_t resident_blocks(int split, int warps, int sm_count) {
-  static std::atomic<int> known[kMaxSplit + 1][kRowsWarps + 1];  // one kind of device: asked once per process
+  static std::atomic<int> known[kMaxSplit + 1][kRowsWarps + 1];  // one more than that; one kind of device: asked once per process
   std::atomic<int>& k = known[split][warps];
-  int n = k.load(std::memory_order_relaxed);
-  if (n) return n;
+  const int before = k.load(std::memory_order_relaxed);
+  if (before) return before - 1;
   auto kern = rows_attn_kernel<HD, MT, BF16>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(split));
@@ -457,35 +455,22 @@ int64_t resident_blocks(int split, int warps, int sm_count) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+  int held = 0;
+  if (cudaOccupancyMaxActiveClusters(&held, kern, &cfg) != cudaSuccess) {
     cudaGetLastError();
-    n = std::max(1, sm_count / split);
+    held = -1;
   }
-  k.store(n * split, std::memory_order_relaxed);
-  return n * split;
+  const int64_t n = slots_held(held, split, sm_count);
+  k.store(int(n) + 1, std::memory_order_relaxed);
+  return n;
 }
 
-struct RowsChoice {
-  int split, warps;
-  int64_t cost;
-};
-// Blocks an item and warps a block: the least (waves of resident blocks) x (chunks a warp walks, and 3 for a block's start and end, one
-// more in a cluster).  us by (warps, blocks): 1x5 rows on 1500 keys (6, 8) 5.5, (8, 4) 5.7, (4, 4) 6.0, (8, 8) 9.2 in two waves; 16x5 on 150..1500
-// (4, 1) 18.1, (6, 1) 17.5, (8, 1) 20.3, (4, 2) 20.6; 64x5 on 258 + 65 (6, 1) 34.4, (2, 1) 38.1, (4, 1) 42.3; 32x5 on 1500 (2, 1) 41.8, (4, 1) 44.9.
 template <int HD, int MT, bool BF16>
-RowsChoice choose_rows(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys, int64_t keys2, int sm_count) {
+RowsChoice choose_for(int64_t B, int64_t R, int G, int n_kv_heads, int64_t keys, int64_t keys2, int sm_count) {
   constexpr int ROWS = 16 * MT, KC = HD == 64 ? 32 : 16;
   const int64_t items = B * n_kv_heads * ((R * G + ROWS - 1) / ROWS);
-  // (32-bit divisions: the loop is host time of every call)
-  const uint32_t blocks = uint32_t(items), chunks = uint32_t(std::min<int64_t>((keys + KC - 1) / KC + std::min<int64_t>((ROWS - 1) / G + 1, R) * ((keys2 + KC - 1) / KC), 1 << 30));
-  RowsChoice best = {1, kRowsWarps, INT64_MAX};
-  for (uint32_t s = 1; s <= uint32_t(kMaxSplit); s *= 2)
-    for (uint32_t w = kRowsWarps; w >= 1; --w) {
-      const uint32_t slots = uint32_t(resident_blocks<HD, MT, BF16>(int(s), int(w), sm_count));
-      const int64_t cost = int64_t((blocks * s + slots - 1) / slots) * ((chunks + s * w - 1) / (s * w) + (s > 1 ? 4 : 3));
-      if (cost < best.cost) best = {int(s), int(w), cost};
-    }
-  return best;
+  const int64_t chunks = std::min<int64_t>((keys + KC - 1) / KC + std::min<int64_t>((ROWS - 1) / G + 1, R) * ((keys2 + KC - 1) / KC), 1 << 30);
+  return choose_rows(uint32_t(items), uint32_t(chunks), [&](int split, int warps) { return resident_blocks<HD, MT, BF16>(split, warps, sm_count); });
 }
 
 template <int HD, int MT, bool BF16>
@@ -503,7 +488,7 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
   p.tiles = (p.R * p.G + ROWS - 1) / ROWS;
   const int64_t items = B * p.Hkv * p.tiles;
   auto kern = rows_attn_kernel<HD, MT, BF16>;
-  const RowsChoice choice = choose_rows<HD, MT, BF16>(B, p.R, p.G, p.Hkv, p.keys, p.k2 ? p.keys2 : 0, sm_count);
+  const RowsChoice choice = choose_for<HD, MT, BF16>(B, p.R, p.G, p.Hkv, p.keys, p.k2 ? p.keys2 : 0, sm_count);
   const int split = choice.split, warps = choice.warps;
   const size_t smem = rows_smem<HD, MT>(warps);
   cudaLaunchConfig_t cfg = {};
@@ -527,9 +512,9 @@ int launch_rows(RowsParams p, int64_t B, int sm_count, cudaStream_t stream) {
 
 // The row kernel's time in us, by its units above: 1.2 each, more with many dimensions or rows to a warp (measured: 1.1 to 1.5, 1.2 to 1.5, 1.6 to 1.75).
 double rows_estimate(int64_t B, int64_t R, int G, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
-  if (hd == 128) return 1.3 * double(choose_rows<128, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
-  if (R * G > 16) return 1.65 * double(choose_rows<64, 2, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
-  return 1.2 * double(choose_rows<64, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
+  if (hd == 128) return 1.3 * double(choose_for<128, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
+  if (R * G > 16) return 1.65 * double(choose_for<64, 2, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
+  return 1.2 * double(choose_for<64, 1, false>(B, R, G, n_kv_heads, keys, keys2, sm_count).cost);
 }
 
 // Whether the tensor-core kernel takes a call, and how it divides it.  Its blocks walk tiles of keys at about 1.15 us each (1.3 where own keys follow),
