@@ -262,8 +262,9 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
         mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
         mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
       }
-      // The reference exponent of a row moves only when its maximum has grown by more than 8 (a weight stays below 2^8).
-      if (__any_sync(0xffffffffu, mx[0] > m[mt][0] + 8.f || mx[1] > m[mt][1] + 8.f)) {
+      // The reference exponent of a row moves only when its maximum has grown by more than that.
+      constexpr float kGrowth = weight_growth(BF16), kLift = weight_lift(BF16);
+      if (__any_sync(0xffffffffu, mx[0] > m[mt][0] + kGrowth || mx[1] > m[mt][1] + kGrowth)) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const float now = fmaxf(m[mt][half], mx[half]), corr = now == m[mt][half] ? 1.f : ex2(m[mt][half] - now);
@@ -276,7 +277,7 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
           }
         }
       }
-      const float base[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0], m[mt][1] == -INFINITY ? 0.f : m[mt][1]};  // (no key of this row yet)
+      const float base[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0] - kLift, m[mt][1] == -INFINITY ? 0.f : m[mt][1] - kLift};  // (no key of this row yet)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll

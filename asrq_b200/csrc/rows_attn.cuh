@@ -20,6 +20,14 @@ struct RowsParams {
   float* parts;
   int n_parts;
 };
+// Both kernels take a row's weights as 2^(s - m + lift), s the scores in units of log 2 and m a maximum that follows s only when s has
+// grown by more than `growth`; the parts' sums and values carry the same 2^lift.  bf16 has the exponents of fp32 and needs no lift.  An fp16
+// weight lies in 2^(growth + lift) = 2^15 at most, all its bits above 2^-14: lifted by 11, weights keep them down to 2^-25 of the largest and count down to 2^-36 of
+// it, so that even 2^24 keys below that would not show in the result.  (Without a lift, weights below 2^-25 of the largest were lost, 40 000 keys of 2^-25 and their
+// thousandth of the result with them.)
+__host__ __device__ constexpr float weight_growth(bool bf16) { return bf16 ? 8.f : 4.f; }
+__host__ __device__ constexpr float weight_lift(bool bf16) { return bf16 ? 0.f : 11.f; }
+
 constexpr int kTcRows = 128, kMaxParts = 64;  // rows of its tile; parts it divides an item's keys into at most
 __host__ __device__ constexpr int part_floats(int hd) { return kTcRows * (hd + 2); }
 

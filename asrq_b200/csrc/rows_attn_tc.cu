@@ -2,13 +2,13 @@
 // states, or the rows of many beams or samples over their prompt.
 //
 // A block holds 128 rows (all query heads of a key head, so several tokens or beams) and walks its keys 96 (64 with 128 dimensions) at a
-// time: S = Q K^T into tensor memory, a thread per row reads its scores, and writes the weights 2^(scale' s - m) in 16 bits to tensor memory
+// time: S = Q K^T into tensor memory, a thread per row reads its scores, and writes the weights 2^(scale' s - m + lift) in 16 bits to tensor memory
 // too, from where O += P V takes them as its first operand.  K arrives by TMA as rows of the contraction, V as it lies, dimensions
 // contiguous, which the second operand's descriptor calls MN-major.  The next S is on its way as soon as the scores are in registers, and
 // two blocks an SM fill each other's waits.  Blocks stay and take one item after the other: the next one's queries and keys arrive and its first S is
 // done while the last weights and the result of the one before are.
-// The reference exponent m of a row moves only when its maximum has grown by more than 8 (a weight stays below 2^8, a sum in 32 bits has
-// room for that): O is scaled at the first tiles and hardly ever after.
+// The reference exponent m of a row moves only when its maximum has grown by more than 8 (bf16; 4 in fp16, see weight_growth): a sum in 32 bits has
+// room for that, and O is scaled at the first tiles and hardly ever after.
 //
 // Bound: at 64 dimensions the exponentials, 16 a cycle and SM, of which every fourth pair goes to the multipliers instead; at 128 these and the
 // memory's bytes where few rows share many keys.
@@ -334,7 +334,7 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
           if (!ok) break;
           tc::fence_after_sync();
         }
-        if (__any_sync(0xffffffffu, high > m + 8.f)) {
+        if (__any_sync(0xffffffffu, high > m + weight_growth(BF16))) {
           const float now = fmaxf(m, high);
           if (j > 0) {
             const float corr = m == now ? 1.f : ex2f(m - now);
@@ -351,7 +351,7 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
           }
           m = now;
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = m == -INFINITY ? 0.f : m - weight_lift(BF16);
         const unsigned long long scale2 = two(p.scale_log2, p.scale_log2), less2 = two(-ref, -ref);
         unsigned long long acc[2] = {0, 0};
 #pragma unroll

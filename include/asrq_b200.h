@@ -340,7 +340,7 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
  *   lengths        B, cut to 0..keys, or NULL for `keys` everywhere; nothing past an utterance's length is read; a row without keys is zero;
  *   out            B x R x n_q_heads x head_dim, contiguous.
  * head_dim 64 or 128; q, k, v, out, workspace and scratch 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation; the weights are
- * rounded to `dtype`.
+ * rounded to `dtype` (in fp16 with all their bits down to 2^-25 of the row's largest, and not at all below 2^-36 of it).
  * Many rows run on the tensor-core kernel, whose waits are bounded: it reports in the workspace's status block (256 bytes, the start of any workspace;
  * asrq_check_status) and, where it divides the keys or the rows have keys of their own, leaves parts in scratch of the call's own
  * (asrq_rows_attention_scratch_bytes says how much, 0 for none; 16-byte aligned, its contents do not matter; as for
