@@ -9,6 +9,8 @@
 // done while the last weights and the result of the one before are.
 // The reference exponent m of a row moves only when its maximum has grown by more than 8 (bf16; 4 in fp16, see weight_growth): a sum in 32 bits has
 // room for that, and O is scaled at the first tiles and hardly ever after.
+// A row's sum is that of the weights as they are rounded, or an average of equal values would not be that value: P times 16 columns of
+// ones, into tensor memory like O (16 x 224 rows on 1500 keys: 56.0 us; 65.9 with threads adding up what they have rounded).
 //
 // Bound: at 64 dimensions the exponentials, 16 a cycle and SM, of which every fourth pair goes to the multipliers instead; at 128 these and the
 // memory's bytes where few rows share many keys.
@@ -38,7 +40,8 @@ struct FlashLayout {
   static constexpr int kKeys = HD == 64 ? 96 : 64;  // of a tile: tensor memory has 256 columns for S (32 bits), P (16 bits) and O of a block
   static constexpr int kStages = HD == 64 ? 3 : 2;
   static constexpr int kQ = kTcRows * HD * 2, kTile = kKeys * HD * 2;
-  static constexpr int kK = kQ, kV = kQ + kStages * kTile, kBars = kQ + 2 * kStages * kTile;
+  static constexpr int kOnesBytes = 2048;  // 16 rows of 128 bytes
+  static constexpr int kK = kQ, kV = kQ + kStages * kTile, kOnes = kQ + 2 * kStages * kTile, kBars = kOnes + kOnesBytes;
   static constexpr int kBytes = kBars + (4 * kStages + 7) * 8 + 16 + 1024;  // 1024: the base is aligned to it
 };
 
@@ -81,6 +84,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
+}
+// one column of tensor memory, 32 lanes of the warp's quadrant
+__device__ __forceinline__ uint32_t tmem_ld_32x1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  return r;
+}
+__device__ __forceinline__ void tmem_st_32x1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
 }
 // registers to tensor memory: 32 lanes of the warp's quadrant x 16 columns
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -139,8 +151,8 @@ __global__ void __launch_bounds__(192, 2)
 flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FlashParams p) {
   using L = FlashLayout<HD>;
   constexpr int ST = L::kStages, HALVES = HD / 64, kKeys = L::kKeys;
-  constexpr uint32_t kP = kKeys, kOut = 256 - HD;  // columns of tensor memory: the scores from 0, the weights, the result
-  static_assert(kP + kKeys / 2 <= kOut, "256 columns");
+  constexpr uint32_t kP = kKeys, kOut = 256 - HD, kSum = kOut - 16;  // columns of tensor memory: the scores from 0, the weights, their sum (16 times), the result
+  static_assert(kP + kKeys / 2 <= kSum, "256 columns");
   extern __shared__ uint8_t flash_smem[];
   const uint32_t base = (tc::smem_u32(flash_smem) + 1023u) & ~1023u;
   uint8_t* smem = flash_smem + (base - tc::smem_u32(flash_smem));
@@ -153,6 +165,11 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
   const uint32_t s_full = bar(4 * ST), s_free = bar(4 * ST + 1), p_full = bar(4 * ST + 2), o_done = bar(4 * ST + 3), q_full = bar(4 * ST + 4), o_free = bar(4 * ST + 5), q_free = bar(4 * ST + 6);
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + L::kBars + (4 * ST + 7) * 8);
 
+  if (threadIdx.x < L::kOnesBytes / 16) {
+    constexpr uint32_t one2 = BF16 ? 0x3f803f80u : 0x3c003c00u;
+    tc::st_shared_v4(base + L::kOnes + threadIdx.x * 16u, one2, one2, one2, one2);
+    tc::fence_proxy_async_smem();
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4 * ST + 7; ++i) {
       const uint32_t x = bar(i);
@@ -246,6 +263,8 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 
   if (warp == 1) {
     const uint32_t s_desc = tc::instr_desc(1, BF16 ? 1 : 0, kTcRows, kKeys), o_desc = tc::instr_desc(1, BF16 ? 1 : 0, kTcRows, HD) | (1u << 16);
+    const uint32_t sum_desc = tc::instr_desc(1, BF16 ? 1 : 0, kTcRows, 16);
+    const uint64_t ones = tc::smem_desc_sw128(base + L::kOnes);
     const bool one = tc::elect_one();
     bool ok = true;
     auto all_wait = [&](uint32_t b, uint32_t parity, unsigned site) { return bool(__all_sync(0xffffffffu, wait(b, parity, p.status, site))); };
@@ -291,6 +310,8 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         tc::fence_after_sync();
         if (one) {
 #pragma unroll
+          for (int x = 0; x < kKeys / 16; ++x) mma_f16_ts(tmem + kSum, tmem + kP + x * 8, ones, sum_desc, j != 0 || x != 0);
+#pragma unroll
           for (int x = 0; x < kKeys / 16; ++x)
             mma_f16_ts(tmem + kOut, tmem + kP + x * 8, smem_desc_mn_sw128(base + L::kV + uint32_t(s * L::kTile + x * 2048), kKeys * 128), o_desc, j != 0 || x != 0);
           tc::mma_commit(o_done);
@@ -307,7 +328,7 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     int t = 0;
     for (int u = int(blockIdx.x); u < p.units && ok; u += step) {
       const Unit w = unit(u);
-      float m = -INFINITY, sum = 0.f;
+      float m = -INFINITY;
       for (int j = 0; j < w.n; ++j, ++t) {
         ok = __all_sync(0xffffffffu, wait(s_full, uint32_t(t) & 1u, p.status, 68));
         if (!ok) break;
@@ -338,7 +359,9 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
           const float now = fmaxf(m, high);
           if (j > 0) {
             const float corr = m == now ? 1.f : ex2f(m - now);
-            sum *= corr;
+            const float sum = __uint_as_float(tmem_ld_32x1(lanes + kSum));
+            tc::tmem_ld_wait();
+            tmem_st_32x1(lanes + kSum, __float_as_uint(sum * corr));
 #pragma unroll
             for (int x = 0; x < HD / 16; ++x) {
               uint32_t o[16];
@@ -353,7 +376,6 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
         const float ref = m == -INFINITY ? 0.f : m - weight_lift(BF16);
         const unsigned long long scale2 = two(p.scale_log2, p.scale_log2), less2 = two(-ref, -ref);
-        unsigned long long acc[2] = {0, 0};
 #pragma unroll
         for (int x = 0; x < kKeys / 32; ++x) {
           uint32_t w16[16];
@@ -368,27 +390,25 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
               asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
               v = two(ex2f(lo), ex2f(hi));
             }
-            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[i % 2]) : "l"(v));
             float lo, hi;
             asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
             w16[i] = pack16<BF16>(lo, hi);
           }
           tmem_st_32x16(lanes + kP + x * 16, w16);
         }
-        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[0]) : "l"(acc[1]));
-        float a0, a1;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc[0]));
-        sum += a0 + a1;
         tc::tmem_st_wait();
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(p_full);
       }
       if (!ok) break;
+      float sum = 0.f;
       if (w.n > 0) {
         ok = __all_sync(0xffffffffu, wait(o_done, uint32_t(t - 1) & 1u, p.status, 70));
         if (!ok) break;
         tc::fence_after_sync();
+        sum = __uint_as_float(tmem_ld_32x1(lanes + kSum));
+        tc::tmem_ld_wait();
       }
       if (m == -INFINITY && sum == sum) sum = 0.f;  // nothing above -inf
       const int rr = w.row0 + r, token = p.G == 1 ? rr : rr / p.G;
