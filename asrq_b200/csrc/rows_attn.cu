@@ -379,9 +379,9 @@ rows_attn_kernel(const __grid_constant__ RowsParams p) {
   auto put4 = [&](int r, int e, float4 v, float mx, float sum) {  // elements e .. e + 3 of the tile's row r
     const int rr = row0 + r;
     if (p.parts) {
-      float* to = p.parts + ((size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + rr / kTcRows) * p.n_parts + p.n_parts - 1) * part_floats(HD);
-      *reinterpret_cast<float4*>(to + (rr % kTcRows) * HD + e) = v;
-      if (e == 0) *reinterpret_cast<float2*>(to + kTcRows * HD + (rr % kTcRows) * 2) = make_float2(mx, sum);
+      const size_t at = ((size_t(bh) * ((p.R * p.G + kTcRows - 1) / kTcRows) + rr / kTcRows) * p.n_parts + p.n_parts - 1) * p.part_rows + rr % kTcRows;
+      *reinterpret_cast<float4*>(p.parts + at * HD + e) = v;
+      if (e == 0) *reinterpret_cast<float2*>(p.stats + at * 2) = make_float2(mx, sum);
       return;
     }
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
@@ -560,15 +560,15 @@ int allow_all() {
   if (!rc) devices.fetch_or(bit, std::memory_order_relaxed);
   return rc;
 }
-size_t part_bytes(int64_t B, int64_t R, int G, int n_kv_heads, int hd, const TcPlan& plan, bool own) {
+size_t part_count(int64_t B, int64_t R, int G, int n_kv_heads, const TcPlan& plan, bool own) {  // rows of all parts
   if (plan.split == 0) return 0;
   const int64_t items = B * n_kv_heads * ((R * G + kTcRows - 1) / kTcRows);
-  return size_t(items - plan.whole) * (plan.split + own) * part_floats(hd) * sizeof(float);
+  return size_t(items - plan.whole) * (plan.split + own) * part_rows_of(R * G);
 }
 
 size_t rows_attention_scratch_bytes(int64_t B, int64_t R, int n_q_heads, int n_kv_heads, int hd, int64_t keys, int64_t keys2, int sm_count) {
   const int G = n_q_heads / n_kv_heads;
-  return allow_all() ? 0 : part_bytes(B, R, G, n_kv_heads, hd, tc_plan(B, R, G, n_kv_heads, hd, keys, keys2, sm_count), keys2 > 0);
+  return allow_all() ? 0 : part_count(B, R, G, n_kv_heads, tc_plan(B, R, G, n_kv_heads, hd, keys, keys2, sm_count), keys2 > 0) * (hd + 2) * sizeof(float);
 }
 
 int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const long long* lengths,
@@ -606,20 +606,21 @@ int rows_attention(const void* q, const int64_t* qs, const void* k, const int64_
   if (status && p.scale_log2 > 0.f && apart(keys, ks[2]) && apart(keys, vs[2]) && apart(B, qs[0]) && apart(R, qs[1]) && apart(n_q_heads, qs[2]))
     plan = tc_plan(B, R, p.G, n_kv_heads, hd, keys, k2 ? keys2 : 0, sm_count);
   if (plan.split > 0) {
-    const size_t need = part_bytes(B, R, p.G, n_kv_heads, hd, plan, k2 != nullptr);
+    const size_t rows = part_count(B, R, p.G, n_kv_heads, plan, k2 != nullptr), need = rows * (hd + 2) * sizeof(float);
     const bool kept = need == 0 || (scratch && scratch_bytes >= need);
     if (!kept && !k2) plan = {B * n_kv_heads * ((R * p.G + kTcRows - 1) / kTcRows), 1};
     if (kept || !k2) {
-      float* parts = need && kept ? static_cast<float*>(scratch) : nullptr;
-      rc = rows_attention_tc(p, hd, bf16, B, plan, parts, k2 ? 1 : 0, status, sm_count, stream);
+      float *parts = need && kept ? static_cast<float*>(scratch) : nullptr, *stats = parts ? parts + rows * hd : nullptr;
+      rc = rows_attention_tc(p, hd, bf16, B, plan, parts, stats, k2 ? 1 : 0, status, sm_count, stream);
       if (!rc && k2) {
         RowsParams own = p;
         own.keys = 0;
-        own.parts = parts;
+        own.parts = parts, own.stats = stats;
         own.n_parts = plan.split + 1;
+        own.part_rows = part_rows_of(R * p.G);
         rc = launch(own);
       }
-      return rc ? rc : rows_attention_join(p, hd, bf16, B, plan.whole, parts, plan.split + (k2 ? 1 : 0), stream);
+      return rc ? rc : rows_attention_join(p, hd, bf16, B, plan.whole, parts, stats, plan.split + (k2 ? 1 : 0), stream);
     }
   }
   return launch(p);

@@ -16,9 +16,9 @@ struct RowsParams {
   int len2_many, R, G, Hkv, tiles;
   float scale_log2;              // scale * log2 e
   // Where the shared keys are the tensor-core kernel's, a row kernel leaves its rows' own keys as one more part: for every utterance, key head and tile of
-  // 128 rows n_parts parts, each 128 x HD values, then 128 pairs of maximum (as an exponent of two) and sum.  The row kernel's is the last.
-  float* parts;
-  int n_parts;
+  // 128 rows n_parts parts of part_rows results of HD values, the row kernel's the last, and in stats as many pairs of maximum (as an exponent of two) and sum.
+  float *parts, *stats;
+  int n_parts, part_rows;
 };
 // Both kernels take a row's weights as 2^(s - m + lift), s the scores in units of log 2 and m a maximum that follows s only when s has
 // grown by more than `growth`; the parts' sums and values carry the same 2^lift.  bf16 has the exponents of fp32 and needs no lift.  An fp16
@@ -29,7 +29,9 @@ __host__ __device__ constexpr float weight_growth(bool bf16) { return bf16 ? 8.f
 __host__ __device__ constexpr float weight_lift(bool bf16) { return bf16 ? 0.f : 11.f; }
 
 constexpr int kTcRows = 128, kMaxParts = 64;  // rows of its tile; parts it divides an item's keys into at most
-__host__ __device__ constexpr int part_floats(int hd) { return kTcRows * (hd + 2); }
+// Rows of a tile's parts: 128, or as many as there are, an odd number: a join reads a row of all parts at once, and at distances of 64 KB they were slower to come
+// (64 samples behind 45 000 keys: 57.7 us for 56.3 with 128 rows for 129).
+__host__ __device__ constexpr int part_rows_of(int64_t rows) { return int(rows < kTcRows ? rows : kTcRows) | 1; }
 
 // How the tensor-core kernel divides a call's items (utterance, key head, 128 rows): the first `whole` have a block each, the keys of the others
 // are divided among `split`, each of which leaves a part.  split 0: the call is not for it.
@@ -39,10 +41,10 @@ struct TcPlan {
 };
 
 // The shared keys of p by tcgen05; room is left behind every item's parts for `more` of them.
-int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, int sm_count,
+int rows_attention_tc(const RowsParams& p, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, float* stats, int more, void* status, int sm_count,
                       cudaStream_t stream);
 
 // The results of the items from `whole` on, from n_parts parts each.
-int rows_attention_join(const RowsParams& p, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, int n_parts, cudaStream_t stream);
+int rows_attention_join(const RowsParams& p, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, const float* stats, int n_parts, cudaStream_t stream);
 
 }  // namespace asrq

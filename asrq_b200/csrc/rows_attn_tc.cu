@@ -15,6 +15,7 @@
 // Bound: at 64 dimensions the exponentials, 16 a cycle and SM, of which every fourth pair goes to the multipliers instead; at 128 these and the
 // memory's bytes where few rows share many keys.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows_attn.cuh"
 
@@ -27,10 +28,10 @@ namespace {
 struct FlashParams {
   uint16_t* out;
   const long long* len;
-  float* parts;
+  float *parts, *stats;  // as in RowsParams
   unsigned* status;
   long long keys;
-  int R, G, Hkv, tiles, units, whole, split, slots, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
+  int R, G, Hkv, tiles, units, whole, split, slots, part_rows, k_batch, v_batch, k_head, v_head;  // *_batch, *_head: 0 where all utterances or heads share them
   // units: what a block takes at a time; the first `whole` are items, the others parts of items, `split` of each; slots: parts of an item there is room for
   float scale_log2;  // positive
 };
@@ -412,7 +413,8 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
       }
       if (m == -INFINITY && sum == sum) sum = 0.f;  // nothing above -inf
       const int rr = w.row0 + r, token = p.G == 1 ? rr : rr / p.G;
-      float* to = w.rest >= 0 ? p.parts + size_t(w.rest) * part_floats(HD) : nullptr;
+      const size_t place = size_t(max(w.rest, 0)) * p.part_rows + r;
+      float* to = w.rest >= 0 ? p.parts + place * HD : nullptr;
       uint16_t* out = p.out + ((size_t(w.b) * p.R + token) * (p.Hkv * p.G) + w.h * p.G + rr - token * p.G) * HD;
       const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
@@ -432,7 +434,7 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
         if (r < w.rows && to) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(to + r * HD + x * 32 + i * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(to + x * 32 + i * 4) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         } else if (r < w.rows) {
           uint32_t w16[16];
 #pragma unroll
@@ -442,7 +444,7 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
         __syncwarp();
       }
-      if (to && r < w.rows) *reinterpret_cast<float2*>(to + kTcRows * HD + r * 2) = make_float2(m, sum);
+      if (to && r < w.rows) *reinterpret_cast<float2*>(p.stats + place * 2) = make_float2(m, sum);
     }
   }
   tc::fence_before_sync();
@@ -454,8 +456,16 @@ flash_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 // take its parts in turn, all loads at once.  Two warps a row up to 16 parts, else eight
 // (16 utterances of 224 rows on 1500 keys, the whole call in us: two 59.8, eight 66.8).
 constexpr int kJoinThreads = 256;
-template <int HD, bool BF16, int WARPS>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float* parts, uint16_t* out, int n_parts, int first_item, int item_blocks, int tiles, int R, int G, int Hkv) {
+// Volatile, or the compiler moves each load whose place it does not know to its use.
+__device__ __forceinline__ float4 load_now(const float* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+// FULL: parts of 128 rows, at distances that the compiler knows (64 samples behind 45 000 keys: 55.9 us for 56.8)
+template <int HD, bool BF16, int WARPS, bool FULL>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const float* parts, const float* stats, uint16_t* out, int n_parts, int rows_of_part, int first_item, int item_blocks, int tiles, int R, int G, int Hkv) {
+  const int part_rows = FULL ? part_rows_of(kTcRows) : rows_of_part;
   constexpr int PER = HD / 4, TEAMS = 32 * WARPS / PER, ROWS = kJoinThreads / (32 * WARPS);  // threads of a part, parts at a time, rows
   constexpr int kMost = WARPS == 2 ? 16 : kMaxParts + 1;
   __shared__ float4 sums[ROWS][TEAMS][PER];
@@ -464,16 +474,17 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float* parts, 
   const int in_block = int(threadIdx.x) / (32 * WARPS), thread = int(threadIdx.x) % (32 * WARPS);
   const int at = int(blockIdx.x) / item_blocks, r = int(blockIdx.x) % item_blocks * ROWS + in_block, item = first_item + at;
   const int rr = (item % tiles) * kTcRows + r;
-  const bool there = rr < R * G;  // (else it reads what nobody wrote, and writes nothing)
+  const bool there = rr < R * G;  // (else it reads what nobody wrote, or another row's, and writes nothing)
   const int lane = threadIdx.x & 31, team = thread / PER, e = (thread % PER) * 4;
-  const float* from = behind_wait(parts + size_t(at) * n_parts * part_floats(HD));
-  const float *ml = from + kTcRows * HD + r * 2, *row = from + r * HD + e;
+  const size_t from = size_t(at) * n_parts * part_rows + min(r, part_rows - 1);  // the row's first part; the others part_rows on each
+  const float *ml = behind_wait(stats + from * 2), *row = behind_wait(parts + from * HD + e);
   constexpr int kEach = (kMost + TEAMS - 1) / TEAMS, kLists = (kMost + 31) / 32;
   float4 o[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int x = i * TEAMS + team;
-    o[i] = x < n_parts ? *reinterpret_cast<const float4*>(row + size_t(x) * part_floats(HD)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (FULL) o[i] = x < n_parts ? *reinterpret_cast<const float4*>(row + x * part_rows * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
+    else o[i] = load_now(row + min(x, n_parts - 1) * part_rows * HD);  // (past the last: it again, not added)
   }
   // every warp: maxima and sums of all parts, two or three a lane
   float2 own[kLists];
@@ -481,7 +492,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const float* parts, 
 #pragma unroll
   for (int i = 0; i < kLists; ++i) {
     const int x = i * 32 + lane;
-    own[i] = x < n_parts ? *reinterpret_cast<const float2*>(ml + size_t(x) * part_floats(HD)) : make_float2(-INFINITY, 0.f);
+    own[i] = x < n_parts ? *reinterpret_cast<const float2*>(ml + x * part_rows * 2) : make_float2(-INFINITY, 0.f);
     mx = fmaxf(mx, own[i].x);
   }
 #pragma unroll
@@ -545,26 +556,30 @@ int launch_flash(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtenso
 
 }  // namespace
 
-int rows_attention_join(const RowsParams& r, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, int n_parts, cudaStream_t stream) {
+int rows_attention_join(const RowsParams& r, int hd, bool bf16, int64_t B, int64_t whole, const float* parts, const float* stats, int n_parts, cudaStream_t stream) {
   const int tiles = (r.R * r.G + kTcRows - 1) / kTcRows;
   const int64_t items = B * r.Hkv * tiles;
   if (whole >= items) return ASRQ_OK;
+  const int part_rows = part_rows_of(int64_t(r.R) * r.G);
   auto go = [&](auto kern, int rows) {
     const int item_blocks = (std::min(r.R * r.G, kTcRows) + rows - 1) / rows;
-    return launch_behind(kern, (items - whole) * item_blocks, kJoinThreads, 0, stream, parts, r.out, n_parts, int(whole), item_blocks, tiles, r.R, r.G, r.Hkv);
+    return launch_behind(kern, (items - whole) * item_blocks, kJoinThreads, 0, stream, parts, stats, r.out, n_parts, part_rows, int(whole), item_blocks, tiles, r.R, r.G, r.Hkv);
   };
-  if (n_parts <= 16) {
-    if (hd == 64) return bf16 ? go(join_kernel<64, true, 2>, 4) : go(join_kernel<64, false, 2>, 4);
-    return bf16 ? go(join_kernel<128, true, 2>, 4) : go(join_kernel<128, false, 2>, 4);
-  }
-  if (hd == 64) return bf16 ? go(join_kernel<64, true, 8>, 1) : go(join_kernel<64, false, 8>, 1);
-  return bf16 ? go(join_kernel<128, true, 8>, 1) : go(join_kernel<128, false, 8>, 1);
+  auto by_rows = [&](auto dim, auto type) {
+    constexpr int HD = decltype(dim)::value;
+    constexpr bool BF16 = decltype(type)::value;
+    const bool full = part_rows == part_rows_of(kTcRows);
+    if (n_parts <= 16) return full ? go(join_kernel<HD, BF16, 2, true>, 4) : go(join_kernel<HD, BF16, 2, false>, 4);
+    return full ? go(join_kernel<HD, BF16, 8, true>, 1) : go(join_kernel<HD, BF16, 8, false>, 1);
+  };
+  if (hd == 64) return bf16 ? by_rows(std::integral_constant<int, 64>{}, std::true_type{}) : by_rows(std::integral_constant<int, 64>{}, std::false_type{});
+  return bf16 ? by_rows(std::integral_constant<int, 128>{}, std::true_type{}) : by_rows(std::integral_constant<int, 128>{}, std::false_type{});
 }
 
-int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, int more, void* status, int sm_count, cudaStream_t stream) {
+int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const TcPlan& plan, float* parts, float* stats, int more, void* status, int sm_count, cudaStream_t stream) {
   FlashParams p = {};
   p.out = r.out, p.len = r.len;
-  p.parts = parts;
+  p.parts = parts, p.stats = stats;
   p.status = static_cast<unsigned*>(status);
   p.keys = r.keys;
   p.R = r.R, p.G = r.G, p.Hkv = r.Hkv;
@@ -572,6 +587,7 @@ int rows_attention_tc(const RowsParams& r, int hd, bool bf16, int64_t B, const T
   p.whole = int(plan.whole);
   p.split = plan.split;
   p.slots = plan.split + more;
+  p.part_rows = part_rows_of(int64_t(p.R) * p.G);
   p.scale_log2 = r.scale_log2;
   p.k_batch = r.k_b != 0, p.v_batch = r.v_b != 0, p.k_head = r.k_h != 0, p.v_head = r.v_h != 0;
   const uint32_t keys = hd == 64 ? FlashLayout<64>::kKeys : FlashLayout<128>::kKeys;
