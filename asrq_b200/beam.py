@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from . import linear as _linear
-from .linear import _expect, _on_device, _require_cuda_16bit, _workspace
+from .linear import _call_scratch, _expect, _on_device, _require_cuda_16bit, _workspace
 
 
 def _ints(t: torch.Tensor, like: torch.Tensor) -> bool:
@@ -99,8 +99,8 @@ def _memory(q: torch.Tensor, key_heads: int, shared: int, own: int):
     """(workspace, its bytes, scratch, its bytes) of a call."""
     ws = _workspace(q.device, _lib.STATUS_BYTES)
     need = int(_lib.load().asrq_rows_attention_scratch_bytes(q.shape[0], q.shape[1], q.shape[2], key_heads, q.shape[3], shared, own))
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    return ws, ws.data_ptr(), ws.numel(), scratch, None if scratch is None else scratch.data_ptr(), need
+    scratch = _call_scratch(need, q.device)
+    return ws, ws.data_ptr(), ws.numel(), scratch, None if scratch is None else scratch.data_ptr(), 0 if scratch is None else need
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor = None, scale: float = None) -> torch.Tensor:

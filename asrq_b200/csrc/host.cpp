@@ -161,10 +161,10 @@ at::Tensor output_like(const at::Tensor& x, int64_t n) {
   return at::detail::empty_cuda(shape, x.scalar_type(), x.device(), std::nullopt);
 }
 
-// Memory of a large call's own for its weights as 16-bit values, from torch's allocator: on a shared stream a block that no other call
-// has, under capture the graph's.  Undefined where the call needs none, and where there is none to be had: the kernels that unpack inside
-// the GEMM run then.
-at::Tensor weights_scratch(int64_t bytes, const c10::Device& device) {
+// Memory of a call's own (a large layer's weights as 16-bit values, the parts of an attention), from torch's allocator: on a shared stream a
+// block that no other call has, under capture the graph's.  Undefined where the call needs none, and where there is none to be had: the
+// kernels that do without run then.
+at::Tensor call_scratch(int64_t bytes, const c10::Device& device) {
   if (bytes == 0) return at::Tensor();
   try {
     return at::detail::empty_cuda({bytes}, at::kByte, device, std::nullopt);
@@ -216,7 +216,7 @@ PyObject* linearq_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     g_calls.fetch_add(1, std::memory_order_relaxed);
     const void* bias = L.bias ? L.bias->data_ptr() : nullptr;
     const int act = gelu ? ASRQ_ACT_GELU : ASRQ_ACT_NONE;
-    const at::Tensor w16 = weights_scratch(int64_t(asrq_linearq_a16_scratch_bytes(m, L.n, L.k, int(L.group), act, bool(res))), x->device());
+    const at::Tensor w16 = call_scratch(int64_t(asrq_linearq_a16_scratch_bytes(m, L.n, L.k, int(L.group), act, bool(res))), x->device());
     rc = asrq_linearq_a16_scratch(int(L.bits), x->data_ptr(), static_cast<const uint8_t*>(L.weight->data_ptr()), L.scales->data_ptr(), L.zeros->data_ptr(),
                                   bias, res ? res->data_ptr() : nullptr, y.data_ptr(), m, L.n, L.k, int(L.group), dtype, act, ws->data_ptr(),
                                   size_t(ws->numel()), w16.defined() ? w16.data_ptr() : nullptr, w16.defined() ? size_t(w16.numel()) : 0, stream);
@@ -433,8 +433,7 @@ bool scale_of(PyObject* o, int64_t hd, float* scale) {
 }
 // Memory of an attention call's own (asrq_rows_attention_scratch_bytes)
 at::Tensor rows_scratch(const at::Tensor& q, int64_t key_heads, int64_t shared, int64_t own) {
-  const size_t n = asrq_rows_attention_scratch_bytes(q.size(0), q.size(1), int(q.size(2)), int(key_heads), int(q.size(3)), shared, own);
-  return n ? at::detail::empty_cuda({int64_t(n)}, at::kByte, q.device(), std::nullopt) : at::Tensor();
+  return call_scratch(int64_t(asrq_rows_attention_scratch_bytes(q.size(0), q.size(1), int(q.size(2)), int(key_heads), int(q.size(3)), shared, own)), q.device());
 }
 inline const int64_t* ints(const at::Tensor* t) { return t ? static_cast<const int64_t*>(t->data_ptr()) : nullptr; }
 

@@ -57,9 +57,9 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     return ws
 
 
-def _weights_scratch(nbytes: int, device: torch.device):
-    """Memory of a large call's own for its weights as 16-bit values (asrq_linearq_a16_scratch): unlike the workspace not shared by
-    what runs on a stream.  None where the call needs none, and where there is none to be had: it then unpacks inside the GEMM."""
+def _call_scratch(nbytes: int, device: torch.device):
+    """Memory of a call's own (asrq_linearq_a16_scratch, asrq_rows_attention_scratch_bytes): unlike the workspace not shared by
+    what runs on a stream.  None where the call needs none, and where there is none to be had: it then runs on kernels that do without."""
     if nbytes == 0:
         return None
     try:
@@ -427,7 +427,7 @@ class LinearQ(nn.Module):
                 r2 = residual.reshape(m, n)
                 r2 = r2 if r2.is_contiguous() else r2.contiguous()
             act = _lib.ACT_GELU if gelu else _lib.ACT_NONE
-            w16 = _weights_scratch(_lib.load().asrq_linearq_a16_scratch_bytes(m, n, k, self.group_size, act, residual is not None), input.device)
+            w16 = _call_scratch(_lib.load().asrq_linearq_a16_scratch_bytes(m, n, k, self.group_size, act, residual is not None), input.device)
             args = (self.bits, x2.data_ptr(), weight.data_ptr(), scales.data_ptr(), zeros.data_ptr(), None if bias is None else bias.data_ptr())
             if w16 is not None:
                 _lib.call("asrq_linearq_a16_scratch", *args, None if r2 is None else r2.data_ptr(), y.data_ptr(), m, n, k, self.group_size, dt, act,

@@ -55,3 +55,41 @@ def test_within_its_bounds(B, R, Hq, Hkv, hd, P, M, dtype):
         assert need > 0 and bool((scratch != 0xFF).any())
     else:
         assert need == 0
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("own", [False, True])
+def test_runs_where_there_is_no_memory_for_it(native, own, monkeypatch):
+    """The allocator has nothing left but the output's memory: the kernels that need no scratch run."""
+    K, H, hd, M = 128, 8, 128, 4
+    B, P = (64, 700) if own else (4, 6000)
+    g = torch.Generator().manual_seed(7)
+    rnd = lambda *shape: torch.randn(*shape, generator=g).half().to(DEV)  # noqa: E731
+    q, k, v, k2, v2, n2 = rnd(B, K, H, hd), rnd(B, H, P, hd), rnd(B, H, P, hd), rnd(B * K, H, M, hd), rnd(B * K, H, M, hd), torch.full((1,), M, device=DEV)
+    if own:
+        call = lambda: asrq_b200.prefix_attention(q, k, v, k2, v2, n2)  # noqa: E731
+    else:
+        call = lambda: asrq_b200.cross_attention(q, k.transpose(1, 2), v.transpose(1, 2))  # noqa: E731
+    if not native:
+        monkeypatch.setattr(asrq_b200.linear, "_native", None)
+    with lib_option("rows_kernel", 2):
+        want, need = call(), _need(B, K, H, H, hd, P, M if own else 0)
+        assert need > (18 << 20)  # more than is left of the allocator's smallest large block, and of what the output's memory is rounded up to
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        block = torch.empty_like(want)  # the output's memory, in the allocator's hands when it is given back
+        total = torch.cuda.get_device_properties(0).total_memory
+        torch.cuda.set_per_process_memory_fraction(torch.cuda.memory_reserved() / total)
+        try:
+            with pytest.raises(torch.OutOfMemoryError):
+                torch.empty(need, dtype=torch.uint8, device=DEV)
+            del block
+            got = call()
+        finally:
+            torch.cuda.set_per_process_memory_fraction(1.0)
+    for out in (want, got):
+        assert torch.equal(out, out) and bool(torch.isfinite(out).all())
+    check_rows(got[:1, ::16].contiguous(), q[:1, ::16], lambda b, r: (torch.cat((k[b], k2[16 * r]), 1).transpose(0, 1), torch.cat((v[b], v2[16 * r]), 1).transpose(0, 1)) if own else
+               (k[b].transpose(0, 1), v[b].transpose(0, 1)))
+    check_rows(want[:1, ::16].contiguous(), q[:1, ::16], lambda b, r: (torch.cat((k[b], k2[16 * r]), 1).transpose(0, 1), torch.cat((v[b], v2[16 * r]), 1).transpose(0, 1)) if own else
+               (k[b].transpose(0, 1), v[b].transpose(0, 1)))
