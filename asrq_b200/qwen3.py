@@ -384,7 +384,7 @@ class Qwen3Engine:
         eos = end_token(self.cfg, eos)
         with torch.cuda.device(self.device):
             self.prefill(inputs_embeds, steps)
-            key = (B, T, steps, beams, eos, self.kc[0].data_ptr())
+            key = (B, T, steps, beams, eos, self.head.shape[0], self.kc[0].data_ptr())
             st = getattr(self, "_beam", None)
             if st is None or st["key"] != key:
                 st = dict(key=key, T=T, beams=BeamState(B, beams, steps, eos, self.device), graph=None, caches=(self.kc, self.vc),

@@ -602,7 +602,7 @@ class WhisperEngine:
                 raise ValueError(f"a prompt {tuple(prompt.shape)} for {b} utterances and {steps} steps in the model's {self.dec_pos.shape[0]} target positions")
             if not 1 <= beams <= 32:
                 raise ValueError(f"{beams} beams (1 to 32)")
-            key = (b, src, beams, t + steps, steps, eos, enc_lengths is not None)
+            key = (b, src, beams, t + steps, steps, eos, enc_lengths is not None, self.head.shape[0])
             st = getattr(self, "_beam", None)
             if st is None or st["key"] != key:
                 hd, nl = self.d // self.heads_d, len(self.dec_layers)
