@@ -602,6 +602,8 @@ class WhisperEngine:
                 raise ValueError(f"a prompt {tuple(prompt.shape)} for {b} utterances and {steps} steps in the model's {self.dec_pos.shape[0]} target positions")
             if not 1 <= beams <= 32:
                 raise ValueError(f"{beams} beams (1 to 32)")
+            if enc_lengths is not None and (not isinstance(enc_lengths, torch.Tensor) or tuple(enc_lengths.shape) != (b,) or enc_lengths.is_floating_point()):
+                raise ValueError(f"enc_lengths: a tensor of {b} whole numbers, got {getattr(enc_lengths, 'dtype', type(enc_lengths))} {tuple(getattr(enc_lengths, 'shape', ()))}")
             key = (b, src, beams, t + steps, steps, eos, enc_lengths is not None, self.head.shape[0])
             st = getattr(self, "_beam", None)
             if st is None or st["key"] != key:

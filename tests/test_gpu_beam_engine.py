@@ -1,4 +1,4 @@
-"""The engines' beam search when something about the engine or the call is not what it was: another output head."""
+"""The engines' beam search when something about the engine or the call is not what it was: another output head, lengths of another shape."""
 import warnings
 
 import pytest
@@ -46,3 +46,11 @@ def test_another_output_head(make, use_graph):
         other.head = head.clone()
         want = other.beam_search(y, 5, 3, eos=7, use_graph=use_graph)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("lengths", [torch.tensor([20]), torch.tensor([[20, 20]]), torch.tensor([20.0, 20.0]), [20, 20]])
+def test_lengths_of_another_shape_or_type(lengths):
+    eng, enc = _whisper()
+    enc = enc[:2]
+    with pytest.raises(ValueError, match="enc_lengths"):
+        eng.beam_search(enc, 4, 3, enc_lengths=lengths)
