@@ -193,7 +193,7 @@ class BeamState:
 
     def start(self, logits: torch.Tensor) -> None:
         """``logits`` (B, V): the K best tokens of every utterance open its beams (the vocabulary has as many)."""
-        scores, parents, tokens = beam_select(logits.view(self.B, 1, -1), torch.zeros(self.B, 1, device=logits.device), self.K)
+        scores, parents, tokens = beam_select(logits.view(self.B, 1, -1), torch.zeros(self.B, 1, dtype=torch.float32, device=logits.device), self.K)
         self.tokens[0], self.parents[0] = tokens, parents
         self.scores.copy_(scores)
         if self.eos is not None:

@@ -1,4 +1,4 @@
-"""The engines' beam search when something about the engine or the call is not what it was: another output head, lengths of another shape."""
+"""The engines' beam search when something about the engine or the call is not what it was: another output head, lengths of another shape, another default type."""
 import warnings
 
 import pytest
@@ -54,3 +54,16 @@ def test_lengths_of_another_shape_or_type(lengths):
     enc = enc[:2]
     with pytest.raises(ValueError, match="enc_lengths"):
         eng.beam_search(enc, 4, 3, enc_lengths=lengths)
+
+
+@pytest.mark.parametrize("make", [_whisper, _qwen3])
+def test_another_default_type(make):
+    """A program that has set torch's default type to 16 bits gets the same search."""
+    eng, x = make()
+    want = eng.beam_search(x, 5, 3, eos=7)
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = eng.beam_search(x, 5, 3, eos=7)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert got[1].dtype == torch.float32 and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
