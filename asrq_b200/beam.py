@@ -29,7 +29,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int = None, finis
     ``scores[b, k] + log_softmax(logits[b, k])[v]``, descending, of equal ones the lowest ``k * V + v``.
 
     ``logits`` (B, K, V) 16-bit with contiguous rows, ``scores`` (B, K) fp32.  Returns ``(scores, parents, tokens)`` of shape (B, n): fp32 and
-    int64, ``parents`` the beam that goes on.  With ``finished`` (B, K) bool and ``eos``: a finished beam goes on with ``eos`` at its own score
+    int64, ``parents`` the beam that goes on.  A beam's normalisation has exponentials of 32 bits (within 4e-6): candidates of different beams that lie nearer than
+    8e-6 may come in either order.  With ``finished`` (B, K) bool and ``eos``: a finished beam goes on with ``eos`` at its own score
     and nothing else, and the fourth result says which of the new hypotheses have ended.  A beam whose score is not finite (at the first
     step all but one) or whose logits are no distribution (a NaN, a +inf, nothing above -inf) offers its tokens at -inf."""
     if _linear._native is not None:  # the ordinary case in native code; None where it is not one

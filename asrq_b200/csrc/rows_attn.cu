@@ -4,7 +4,8 @@
 //   prefix   the rows are beams or samples that share a prompt's keys; behind these each has its own.
 //
 // out[row] = sum_t w_t v_t / sum_t w_t, w_t = exp(scale q . k_t - m) over the row's keys, in one pass with the running maximum m
-// and sum.  A row without keys is zero.  fp32 scores, softmax and accumulation.
+// and sum.  A row without keys is zero.  fp32 scores, softmax and accumulation; the weights are rounded to the values' type, which the second product
+// takes, and the sum is that of the rounded ones.
 //
 // Bound: the bytes of the keys and values, read once for up to 16 rows (32 with heads of 64) of a key head.  A warp takes a chunk of
 // 32 keys (16 with heads of 128) at a time, all dimensions, and keeps the rows' results in registers; the chunks of an item (utterance, key

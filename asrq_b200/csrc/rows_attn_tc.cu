@@ -9,6 +9,8 @@
 // done while the last weights and the result of the one before are.
 // The reference exponent m of a row moves only when its maximum has grown by more than 8 (bf16; 4 in fp16, see weight_growth): a sum in 32 bits has
 // room for that, and O is scaled at the first tiles and hardly ever after.
+// The weights are rounded to the values' type, which is what the second product takes (a second one of their remainders would double it): half a step
+// each, against which the polynomial's 2.6e-6 does not count.
 // A row's sum is that of the weights as they are rounded, or an average of equal values would not be that value: P times 16 columns of
 // ones, into tensor memory like O (16 x 224 rows on 1500 keys: 56.0 us; 65.9 with threads adding up what they have rounded).
 //

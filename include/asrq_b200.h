@@ -307,8 +307,9 @@ int asrq_decode_grouped_attention(const void* qkv, const void* q_weight, const v
 /*
  * Decoding with several hypotheses (beams) per utterance: the selection of a step.  Over the K beams and V tokens of an utterance
  *   s[k, v] = scores[k] + logits[k, v] - log sum_v' exp logits[k, v'],
- * and the n largest with their beam (parents) and token, descending, of equal ones the lowest k * V + v first (the logits of a beam decide
- * before s is rounded).  s is computed in 64 bits and returned in 32.
+ * and the n largest with their beam (parents) and token, descending, of equal ones the lowest k * V + v first.  s is put together in 64 bits and returned
+ * in 32, but the exponentials under the logarithm are of 32 bits: a beam's normalisation is within 4e-6 of the exact one.  So continuations of one beam come in the order of their logits, always; beams with the same logits and score tie; continuations
+ * of different beams that differ by less than 8e-6 may come in either order, the same one in every call.
  *   logits      beam k of utterance b at logits + b * utterance_stride + k * beam_stride, V contiguous values of `dtype`, at any value's address;
  *   scores      B x K; a beam whose score is not finite is no hypothesis: its continuations have -inf (at the first step all but one beam);
  *               so has one whose logits hold a NaN, a +inf or nothing above -inf;
@@ -337,11 +338,13 @@ int asrq_beam_reorder(void* cache, const int64_t* parents, const int64_t* length
  * Attention of R query rows of every utterance (the beams of a step, the tokens of a prompt) over its encoder states:
  * out[b, r, h] = softmax(scale * q[b, r, h] . k[b, t, h'])_t . v[b, t, h'], t < lengths[b], h' = h / (n_q_heads / n_kv_heads).
  *   q, q_strides   values between utterances, rows and heads;  k, v and theirs: between utterances, heads and positions; multiples of 8;
- *   lengths        B, cut to 0..keys, or NULL for `keys` everywhere; nothing past an utterance's length is read; a row without keys is zero;
+ *   lengths        B, cut to 0..keys, or NULL for `keys` everywhere; what lies past an utterance's length does not matter (within `keys` it may be read); a row
+ *                  without keys is zero;
  *   out            B x R x n_q_heads x head_dim, contiguous.
  * head_dim 64 or 128; q, k, v, out, workspace and scratch 16-byte aligned; any R.  The strides are read during the call.  fp32 scores, softmax and accumulation; the weights are
- * rounded to `dtype` (in fp16 with all their bits down to 2^-25 of the row's largest, and not at all below 2^-36 of it).
- * Many rows run on the tensor-core kernel, whose waits are bounded: it reports in the workspace's status block (256 bytes, the start of any workspace;
+ * rounded to `dtype`, and a row's sum is that of the rounded ones (in fp16 with all their bits down to 2^-25 of the row's largest, and not at all below 2^-36 of it).
+ * Many rows (n_q_heads / n_kv_heads of them for each r) run on the tensor-core kernel where that group divides 128; where it does not (3, 5, 6, 7, 12), on
+ * the kernel for few rows, which takes two to four times as long for 64 rows and more in large batches.  The tensor-core kernel's waits are bounded: it reports in the workspace's status block (256 bytes, the start of any workspace;
  * asrq_check_status) and, where it divides the keys or the rows have keys of their own, leaves parts in scratch of the call's own
  * (asrq_rows_attention_scratch_bytes says how much, 0 for none; 16-byte aligned, its contents do not matter; as for
  * asrq_linearq_a16_scratch it belongs to this call alone until its work is done).  Without a workspace, or without the scratch, other kernels run.
